@@ -186,6 +186,70 @@ int soapmi_row_major_to_col_major_f32(const float* in, int64_t ldi, float* out, 
 int soapmi_col_major_to_row_major_f32(const float* in, int64_t ldi, float* out, int64_t ldo, int64_t rows,
                                       int64_t cols, void* stream);
 
+/* ---- products of the layers whose weights are trained ----------------------------------------
+ *
+ * No counterpart in the reference, which starts from a gradient; these are the products that a
+ * layer's forward and backward pass are made of, up to the gradient matrix that the calls above take.
+ * Matrices here are row-major, as torch keeps them: element (i, j) at p[i * ld + j].  Rows of x, y and
+ * their gradients are tokens, sorted by expert: expert e has the rows ends[e-1] .. ends[e]-1 (0 before
+ * the first), `ends` being `experts` ascending int64 values on the device, at most `tokens`; it may be
+ * NULL for one expert that has every row.  An expert may have no row.  Sizes stay on the device: no
+ * call synchronises, needs a workspace or depends on where the rows are cut, and all of them can be
+ * captured into a graph and replayed with other values in `ends`.  Values of `ends` that are not
+ * ascending or not in 0 .. tokens are held to that range, so every access stays inside the buffers,
+ * but which rows are then computed is not specified.  A weight matrix is n x k (outputs x inputs);
+ * expert e's starts e * stride elements after the first.  `dtype` and `out_dtype` are one of the
+ * SOAPMI_FLOAT32, SOAPMI_BFLOAT16, SOAPMI_FLOAT16; sums are formed in fp32 on the matrix cores (8-bit
+ * codes: exactly, in 32-bit integers) and rounded once.  Results do not depend on scheduling.
+ * tokens, n, k < 2^30.  Buffers of one call must not overlap, except where it says so. */
+#define SOAPMI_FLOAT32 0
+#define SOAPMI_BFLOAT16 1
+#define SOAPMI_FLOAT16 2
+
+/* transposed == 0: y[t, :] = W_e x[t, :]   (x: tokens x k, y: tokens x n; the forward product);
+ * transposed != 0: y[t, :] = W_e^T x[t, :] (x: tokens x n, y: tokens x k; the input's gradient).
+ * out_dtype is dtype or SOAPMI_FLOAT32.  Rows behind the last expert's are left as they were, or set to
+ * zero where zero_rest != 0. */
+int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t stride_w,
+                          int transposed, const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
+                          int out_dtype, void* y, int64_t ldy, int zero_rest, void* stream);
+
+/* dW_e (n x k) = sum over e's rows t of gradient[t, :]^T x[t, :]; zeros for an expert without rows.
+ * gradient: tokens x n, x: tokens x k, both of `dtype`; out_dtype is dtype or SOAPMI_FLOAT32. */
+int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, const void* x, int64_t ldx,
+                                  const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
+                                  int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* stream);
+
+/* The same with x as soapmi_checkpoint_activations saved it from values of `dtype` (16-bit types only: a
+ * fp32 checkpoint is restored first).  The codes' steps are powers of two, so x enters the product
+ * exactly as it is restored. */
+int soapmi_expert_weight_gradient_saved(int dtype, const void* gradient, int64_t ldg, const int8_t* codes, int64_t ldq,
+                                        const uint8_t* exponents, int64_t lde, const int64_t* ends, int64_t experts,
+                                        int64_t tokens, int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw,
+                                        int64_t stride_dw, void* stream);
+
+/* Activation checkpoint of a rows x cols matrix: 8-bit codes (rows x cols) and an exponent for each row
+ * and 128 columns (rows x ceil(cols / 128)).  With 2^(p-1) <= m < 2^p the largest magnitude of those
+ * columns, step = 2^max(p-7, -126) (fp16: 2^max(p-7, -24)), code = round-to-even(x / step) held to
+ * -127..127, exponent = log2(step) + 127.  A value is restored as code * step, off by at most half a step
+ * (one step above 127.5 steps).  Columns that hold an infinity or NaN get exponent 255 and are restored as NaN. */
+int soapmi_checkpoint_activations(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes,
+                                  int64_t ldq, uint8_t* exponents, int64_t lde, void* stream);
+int soapmi_restore_activations(int dtype, const int8_t* codes, int64_t ldq, const uint8_t* exponents, int64_t lde,
+                               int64_t rows, int64_t cols, void* x, int64_t ldx, void* stream);
+
+/* 8-bit codes of a matrix's rows (tokens, or a weight's output channels): scale = m / 127 with m the row's
+ * largest magnitude, code = round-to-even(127 x / m) in -127..127.  A row of zeros has scale 0; a row that
+ * holds an infinity or NaN has scale NaN and codes 0. */
+int soapmi_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldq,
+                         float* scales, void* stream);
+
+/* y[t, j] = scales[t] * w_scales[j] * sum over i of codes[t, i] * w_codes[j, i]; codes: tokens x k, w_codes:
+ * n x k, k <= 131071 (the integer sum stays inside 32 bits), y: tokens x n. */
+int soapmi_int8_product(const int8_t* codes, int64_t ldq, const float* scales, const int8_t* w_codes, int64_t ldw,
+                        const float* w_scales, int64_t tokens, int64_t n, int64_t k, int out_dtype, void* y, int64_t ldy,
+                        void* stream);
+
 /* ---- basis refresh ------------------------------------------------------------------------ */
 
 /* work <- A Q for the symmetric n x n matrix A (both triangles must be valid).  Replaces

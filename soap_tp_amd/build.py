@@ -9,6 +9,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -19,7 +21,7 @@ INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 # hardware-counter runs, where the profiled program should be a plain executable).
 ABI_PROBE_SOURCE = PACKAGE_DIR.parent / "tests" / "native" / "abi_probe.cpp"
 ABI_PROBE_PATH = PACKAGE_DIR.parent / "tests" / "native" / "abi_probe.bin"
-SOURCES = ("api.hip",)
+SOURCES = ("api.hip", "products.hip", "products_bf16.hip", "products_f16.hip", "products_i8.hip")
 
 # -packed-fp32-ops is switched off on purpose: the compiler must not fuse scalar fp32 code
 # into v_pk_* instructions on this target.
@@ -28,7 +30,6 @@ HIPCC_FLAGS = (
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Wno-unused-result",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 )
@@ -41,10 +42,7 @@ def hipcc_path() -> str:
     return found
 
 
-def build(verbose: bool = False) -> Path:
-    command = [hipcc_path(), *HIPCC_FLAGS]
-    command += [str(CSRC_DIR / source) for source in SOURCES]
-    command += ["-o", str(LIBRARY_PATH)]
+def _run(command, verbose: bool) -> None:
     if verbose:
         print(" ".join(command), flush=True)
     completed = subprocess.run(command, capture_output=True, text=True)
@@ -54,6 +52,18 @@ def build(verbose: bool = False) -> Path:
         raise RuntimeError(f"hipcc failed ({completed.returncode}):\n{stderr}")
     if verbose and stderr.strip():
         print(stderr, file=sys.stderr)
+
+
+def build(verbose: bool = False) -> Path:
+    """Compile the sources side by side and link them."""
+    hipcc = hipcc_path()
+    with tempfile.TemporaryDirectory(prefix="soap_mi355_") as folder:
+        objects = [str(Path(folder) / f"{Path(source).stem}.o") for source in SOURCES]
+        commands = [[hipcc, *HIPCC_FLAGS, "-c", str(CSRC_DIR / source), "-o", target]
+                    for source, target in zip(SOURCES, objects)]
+        with ThreadPoolExecutor(max_workers=min(len(commands), os.cpu_count() or 1)) as pool:
+            list(pool.map(lambda command: _run(command, verbose), commands))
+        _run([hipcc, "--offload-arch=gfx950", "-shared", *objects, "-o", str(LIBRARY_PATH)], verbose)
     return LIBRARY_PATH
 
 

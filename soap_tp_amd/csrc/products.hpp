@@ -1,0 +1,865 @@
+// Products of a layer with weights grouped by expert, in 16-bit floating point and 8-bit integers.
+//
+//   rows grouped (forward, input gradient):  Y[t, c] = sum_k R[t, k] C_e(t)[c, k]
+//   k grouped    (weight gradient):          D_e[r, c] = sum over t in e of R[t, r] C[t, c]
+//
+// The rows t of expert e are [ends[e-1], ends[e]).  The sizes are only known on the device: a launch
+// has as many workgroups as the worst split of the rows can need, every workgroup finds its tile from
+// `ends` itself (a prefix sum over the experts in one wavefront's lanes), and the ones behind the last
+// tile leave.  Nothing is read back to the host and no launch prepares another.
+//
+// Operands.  Each operand is KC (its k index is contiguous in memory) or XC (its row or column index
+// is).  A slab of 128 bytes of k (KC: 64 16-bit or 128 8-bit values; XC: 64 values) is kept in LDS
+// twice, so that the next one travels while this one is multiplied:
+//   KC  S[x][128 bytes], 16-byte pieces, piece p of row x stored at p ^ key(x): the 16 rows that a
+//       fragment read touches then start in different banks;
+//   XC  S[k][x], 32-byte blocks, block b of row k stored at b ^ f(k); fragments are read with the
+//       transposing LDS read, which hands each lane 4 consecutive k of one x.
+// Both layouts are linear in the order in which lanes fetch, which is what a load from memory straight
+// to LDS needs: the permutation is applied to the address each lane fetches from.
+//
+// The matrix instruction's first operand is the column side, so that a lane's accumulators are
+// consecutive columns of one output row; columns are dealt to fragments in such a way that two
+// fragments give a lane eight consecutive ones (one 16-byte store of 16-bit results).
+#pragma once
+#include "common.hpp"
+#include "gemm.hpp"
+
+namespace soapmi {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+enum : int { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };  // SOAPMI_FLOAT32 ...
+
+struct ElemBF16 {
+  static constexpr int SIZE = 2;
+  using Acc = f32x4;
+  using Scalar = __bf16;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+struct ElemF16 {
+  static constexpr int SIZE = 2;
+  using Acc = f32x4;
+  using Scalar = _Float16;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+struct ElemI8 {
+  static constexpr int SIZE = 1;
+  using Acc = i32x4;
+  using Scalar = int8_t;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+};
+
+// ---- which tile a workgroup has ------------------------------------------------------------
+
+struct RowGroups {
+  const int64_t* ends;  // null: one expert holds every row
+  int experts;
+  int rest;             // rows behind the last expert's are a group of their own (written as zeros)
+  int tokens;
+};
+
+// Group g's rows.  Whatever `ends` holds, they lie in [0, tokens).
+__device__ __forceinline__ void group_rows(const RowGroups& g, int e, int& begin, int& end) {
+  if (g.ends == nullptr) {
+    begin = e == 0 ? 0 : g.tokens;
+    end = g.tokens;
+    return;
+  }
+  const int64_t lo = e > 0 ? g.ends[e - 1] : 0, hi = e < g.experts ? g.ends[e] : g.tokens;
+  begin = (int)min(max(lo, (int64_t)0), (int64_t)g.tokens);
+  end = max(begin, (int)min(max(hi, (int64_t)0), (int64_t)g.tokens));
+}
+
+__device__ __forceinline__ int wave_inclusive_sum(int v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
+struct RowTile {
+  int expert;  // == experts: the rest
+  int row;     // first row
+  int rows;    // rows of the tile that belong to the group (1 .. BR)
+};
+
+// Tile number wg of the launch -> its rows and columns.  Row tiles never cross a group's end.
+// Consecutive workgroup ids are dealt round-robin to the 8 XCDs; each XCD gets one contiguous range of
+// tiles, walked in groups of up to 8 row tiles by all columns, so that a weight tile is fetched into
+// that XCD's L2 once for its row tiles.  Returns false behind the last tile.
+template <int BR>
+__device__ __forceinline__ bool locate_rows(const RowGroups& g, int tiles_c, int wg, RowTile& tile, int& tile_c) {
+  const int lane = threadIdx.x & 63;
+  const int groups = g.experts + g.rest;
+  int total = 0;
+  int first_tiles = 0, first_begin = 0, first_end = 0;  // of the first 64 groups, kept for the search
+  for (int e0 = 0; e0 < groups; e0 += 64) {
+    int begin = 0, end = 0;
+    if (e0 + lane < groups) group_rows(g, e0 + lane, begin, end);
+    const int tiles = wave_inclusive_sum((end - begin + BR - 1) / BR, lane);
+    if (e0 == 0) {
+      first_tiles = tiles;
+      first_begin = begin;
+      first_end = end;
+    }
+    total += __shfl(tiles, 63);
+  }
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int64_t all = (int64_t)total * tiles_c;
+  const int64_t chunk = (all + 7) >> 3;
+  const int64_t t = (int64_t)(wg & 7) * chunk + (wg >> 3);
+  if ((wg >> 3) >= chunk || t >= all) return false;
+  constexpr int GR = 8;
+  const int64_t per = (int64_t)GR * tiles_c;
+  const int band = (int)(t / per), in_band = (int)(t - band * per);
+  const int rows = min(GR, total - band * GR);
+  const int tr = band * GR + in_band % rows;
+  tile_c = in_band / rows;
+  int before = 0;
+  for (int e0 = 0; e0 < groups; e0 += 64) {
+    int begin = first_begin, end = first_end, tiles = first_tiles;
+    if (e0 > 0) {
+      begin = end = 0;
+      if (e0 + lane < groups) group_rows(g, e0 + lane, begin, end);
+      tiles = wave_inclusive_sum((end - begin + BR - 1) / BR, lane);
+    }
+    const uint64_t behind = __ballot(before + tiles > tr);
+    if (behind) {
+      const int at = __ffsll((unsigned long long)behind) - 1;
+      const int up_to = at ? __shfl(tiles, at - 1) : 0;
+      begin = __shfl(begin, at);
+      end = __shfl(end, at);
+      tile.expert = __builtin_amdgcn_readfirstlane(e0 + at);
+      tile.row = __builtin_amdgcn_readfirstlane(begin + (tr - before - up_to) * BR);
+      tile.rows = __builtin_amdgcn_readfirstlane(min(BR, end - (begin + (tr - before - up_to) * BR)));
+      return true;
+    }
+    before += __shfl(tiles, 63);
+  }
+  return false;  // (not reached: tr < total)
+}
+
+// ---- operands ------------------------------------------------------------------------------
+
+// Address bits that spread KC rows over the banks.  The row side reads rows x .. x+15; the column side
+// reads rows 8g + {0..3} (+ 4) for g = 0..3, see column_of.
+__device__ __forceinline__ int kc_key(bool column_side, int x) {
+  return column_side ? (x & 3) | ((x >> 1) & 4) : x & 7;
+}
+// ... and XC rows: a transposing read of 32 lanes covers k rows {0..3, 8..11} (+ 4).
+template <int BX>
+__device__ __forceinline__ int xc_key(int k) {
+  return ((k & 3) | ((k >> 1) & 4)) & (BX / 16 - 1);
+}
+
+// Columns of a wavefront's fragment i, row m of the matrix instruction: fragments 2i and 2i+1 give lane
+// group g (m / 4) the columns 32i + 8g .. 32i + 8g + 7.
+__device__ __forceinline__ int column_of(int i, int m) { return 32 * (i >> 1) + 8 * (m >> 2) + 4 * (i & 1) + (m & 3); }
+
+enum Layout { KC, XC };
+// How an operand gets to LDS.  Direct: 16-byte pieces straight from memory (aligned operands).  Staged:
+// through registers, any alignment and size.  Codes: through registers, 8-bit codes of an activation
+// checkpoint expanded to 16-bit values on the way.
+enum Source { Direct, Staged, Codes };
+
+struct Operand {
+  const char* base;  // tile's first element
+  int64_t ld;        // bytes from one stored row to the next
+  int valid;         // rows (columns) of the tile that exist
+  // Codes only: exponents[k * ld_exp], of the tile's first row and first block
+  const uint8_t* exponents;
+  int64_t ld_exp;
+};
+
+constexpr unsigned kOutside = 0xC0000000u;    // a byte offset outside every buffer: such a lane fetches zeros
+constexpr int kBufferBytes = 0x40000000;
+
+// 16 bytes per lane from memory to LDS at lds + 16 * lane (lds: the same in all lanes of a wavefront).
+// In inline assembly because the compiler, told of such a load, waits for it before every transposing
+// LDS read, the ones of the other buffer included.  There is no output register; the waits are
+// wait_direct().
+__device__ __forceinline__ void load_to_lds(i32x4 resource, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(offset), "s"(resource)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void wait_direct() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ i32x4 buffer_of(const char* base) {
+  const uint64_t address = reinterpret_cast<uint64_t>(base);
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)address);
+  r[1] = __builtin_amdgcn_readfirstlane((int)((address >> 32) & 0xffff));
+  r[2] = kBufferBytes;
+  r[3] = 0x00020000;
+  return r;
+}
+
+__device__ __forceinline__ i32x4 load_bytes(const char* p, int count) {
+  i32x4 v = {0, 0, 0, 0};
+  if (count >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else if (count > 0) {
+    char b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = i < count ? p[i] : 0;
+    __builtin_memcpy(&v, b, 16);
+  }
+  return v;
+}
+
+__device__ __forceinline__ float exponent_value(int code) {  // 2^(code - 127); 255: not a number
+  return __uint_as_float(code == 255 ? 0x7fc00000u : (unsigned)code << 23);
+}
+
+// One operand of a tile: BX rows (or columns), slabs of 128 bytes (KC) or 64 values (XC) of k.
+template <class E, Layout L, Source S, int BX, int NT, bool COLUMN>
+struct Loader {
+  static constexpr int SLAB_K = L == KC ? 128 / E::SIZE : 64;
+  static constexpr int BYTES = L == KC ? BX * 128 : 64 * BX * E::SIZE;
+  static constexpr int PIECES = BYTES / 16;
+  static constexpr int NP = (PIECES + NT - 1) / NT;
+  static_assert(L == KC || E::SIZE == 2, "transposing reads are of 16-bit values");
+  static_assert(S != Codes || L == XC, "codes are expanded along x");
+  static_assert(S != Direct || PIECES % 64 == 0, "whole wavefronts fetch");
+  static constexpr int PER_ROW = L == KC ? 8 : BX * E::SIZE / 16;  // pieces in an LDS row
+
+  const char* base;
+  int64_t ld;
+  int valid;
+  const uint8_t* exponents;
+  int64_t ld_exp;
+  int tid;
+  unsigned offset[S == Direct ? NP : 1];
+  i32x4 held[S == Direct ? 1 : NP];
+  int held_exp[S == Codes ? NP : 1];
+
+  // stored row and piece of LDS piece q
+  static __device__ __forceinline__ void place(int q, int& row, int& piece) {
+    row = q / PER_ROW;
+    const int slot = q % PER_ROW;
+    if (L == KC) piece = slot ^ kc_key(COLUMN, row);
+    else piece = (((slot >> 1) ^ xc_key<BX>(row)) << 1) | (slot & 1);
+  }
+
+  __device__ __forceinline__ void init(const Operand& o, int tid_) {
+    base = o.base;
+    ld = o.ld;
+    valid = o.valid;
+    exponents = o.exponents;
+    ld_exp = o.ld_exp;
+    tid = tid_;
+    if constexpr (S == Direct) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        int row, piece;
+        place(tid + i * NT, row, piece);
+        // (rows behind the tile's last one are fetched as its last one again: they only reach
+        // output rows that are not stored; columns behind it as zeros)
+        if (L == KC) offset[i] = (unsigned)(min(row, valid - 1) * (int)ld + piece * 16);
+        else offset[i] = piece * 16 / E::SIZE < valid ? (unsigned)(row * (int)ld + piece * 16) : kOutside;
+      }
+    }
+  }
+
+  // Starts fetching slab kt; k_left = values of k from this slab on.
+  __device__ __forceinline__ void fetch(int kt, int k_left, unsigned lds) {
+    const char* at = L == KC ? base + (int64_t)kt * 128 : base + (int64_t)kt * 64 * ld;
+    if constexpr (S == Direct) {
+      const i32x4 resource = buffer_of(at);
+      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (PIECES % NT != 0 && (wave + i * (NT / 64)) * 64 >= PIECES) break;
+        int row, piece;
+        place(tid + i * NT, row, piece);
+        const bool inside = L == KC ? piece * 16 < k_left * E::SIZE : row < k_left;
+        load_to_lds(resource, inside ? offset[i] : kOutside, lds + (wave * 64 + i * NT) * 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int q = tid + i * NT;
+        if (PIECES % NT != 0 && q >= PIECES) break;
+        int row, piece;
+        place(q, row, piece);
+        if constexpr (S == Staged) {
+          if (L == KC) {
+            const int r = min(row, valid - 1);
+            held[i] = load_bytes(at + r * ld + piece * 16, k_left * E::SIZE - piece * 16);
+          } else {
+            held[i] = row < k_left ? load_bytes(at + row * ld + piece * 16, valid * E::SIZE - piece * 16) : i32x4{0, 0, 0, 0};
+          }
+        } else {
+          // eight codes for a piece of eight 16-bit values
+          const int count = row < k_left ? valid - piece * 8 : 0;
+          held[i] = i32x4{0, 0, 0, 0};
+          held_exp[i] = 0;
+          if (count > 0) {
+            const char* p = at + row * ld + piece * 8;
+            held_exp[i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (piece >> 4)];
+            if (count >= 8) {
+              __builtin_memcpy(&held[i], p, 8);
+            } else {
+              char b[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
+              __builtin_memcpy(&held[i], b, 8);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // Staged and Codes: what fetch() brought goes to LDS.
+  __device__ __forceinline__ void put(char* lds) {
+    if constexpr (S != Direct) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int q = tid + i * NT;
+        if (PIECES % NT != 0 && q >= PIECES) break;
+        if constexpr (S == Staged) {
+          *reinterpret_cast<i32x4*>(lds + q * 16) = held[i];
+        } else {
+          // code * 2^e is exact in bf16 (8 bits of mantissa) and, with the exponents that
+          // checkpoints of fp16 values have, in fp16
+          const float step = exponent_value(held_exp[i]);
+          typename E::Scalar v[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            v[j] = (typename E::Scalar)((float)(int8_t)((unsigned)held[i][j >> 2] >> (8 * (j & 3))) * step);
+          __builtin_memcpy(lds + q * 16, v, 16);
+        }
+      }
+    }
+  }
+
+  // 16 bytes of fragment data for (x, k step ks): KC: k pieces 4 ks + lane group; XC: 8 k values.
+  // x0: first x of the wavefront, i: fragment.
+  static __device__ __forceinline__ i32x4 fragment(const char* lds, int x0, int i, int ks, int lane) {
+    const int m = lane & 15, g = lane >> 4;
+    if constexpr (L == KC) {
+      const int x = x0 + (COLUMN ? column_of(i, m) : 16 * i + m);
+      return *reinterpret_cast<const i32x4*>(lds + x * 128 + (((ks * 4 + g) ^ kc_key(COLUMN, x)) << 4));
+    } else {
+      // lane m of a 16-lane group supplies four x (chunk m % 4) of k row m / 4 and receives column m
+      const int x = x0 + (COLUMN ? 32 * (i >> 1) + 8 * (m & 3) + 4 * (i & 1) : 16 * i + 4 * (m & 3));
+      i32x4 out;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = ks * 32 + g * 8 + h * 4 + (m >> 2);
+        char* p = const_cast<char*>(lds) + k * (BX * E::SIZE) + ((((x >> 4) ^ xc_key<BX>(k)) << 5) | ((x & 15) << 1));
+        const s16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)p);
+        const auto two = __builtin_bit_cast(int __attribute__((ext_vector_type(2))), part);
+        out[2 * h] = two[0];
+        out[2 * h + 1] = two[1];
+      }
+      return out;
+    }
+  }
+};
+
+template <int BR_, int BC_, int WR_, int WC_>
+struct ProductTile {
+  static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_;
+  static constexpr int NT = 64 * WR * WC;
+  static constexpr int TR = BR / WR / 16, TC = BC / WC / 16;
+  static_assert(TC % 2 == 0, "columns are dealt to pairs of fragments");
+  static_assert(BR % (16 * WR) == 0 && BC % (16 * WC) == 0, "wave tiling");
+};
+
+// acc = sum over k of R[r, k] C[c, k] of one tile.
+template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg>
+struct TileProduct {
+  using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false>;
+  using LoadC = Loader<E, LC, SC, Cfg::BC, Cfg::NT, true>;
+  static constexpr int SLAB_K = LoadR::SLAB_K;
+  static_assert(LoadR::SLAB_K == LoadC::SLAB_K, "one slab for both operands");
+  static constexpr int STAGE = LoadR::BYTES + LoadC::BYTES;
+  static constexpr int LDS_BYTES = 2 * STAGE;
+  using Acc = typename E::Acc;
+
+  static __device__ __forceinline__ void run(const Operand& r, const Operand& c, int k_count, char* lds,
+                                             Acc (&acc)[Cfg::TR][Cfg::TC]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wr0 = (wave % Cfg::WR) * (Cfg::TR * 16), wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
+#pragma unroll
+    for (int j = 0; j < Cfg::TR; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::TC; ++i) acc[j][i] = Acc{0, 0, 0, 0};
+    const int slabs = (k_count + SLAB_K - 1) / SLAB_K;
+    if (slabs == 0) return;
+    const unsigned lds_address = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    LoadR lr;
+    LoadC lc;
+    lr.init(r, tid);
+    lc.init(c, tid);
+    lr.fetch(0, k_count, lds_address);
+    lc.fetch(0, k_count, lds_address + LoadR::BYTES);
+    lr.put(lds);
+    lc.put(lds + LoadR::BYTES);
+    wait_direct();
+    __syncthreads();
+    for (int kt = 0; kt < slabs; ++kt) {
+      const int here = (kt & 1) * STAGE, next = STAGE - here;
+      const bool more = kt + 1 < slabs;
+      if (more) {
+        lr.fetch(kt + 1, k_count - (kt + 1) * SLAB_K, lds_address + next);
+        lc.fetch(kt + 1, k_count - (kt + 1) * SLAB_K, lds_address + next + LoadR::BYTES);
+      }
+      const char* sr = lds + here;
+      const char* sc = sr + LoadR::BYTES;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4 fr[Cfg::TR], fc[Cfg::TC];
+#pragma unroll
+        for (int i = 0; i < Cfg::TC; ++i) fc[i] = LoadC::fragment(sc, wc0, i, ks, lane);
+#pragma unroll
+        for (int j = 0; j < Cfg::TR; ++j) fr[j] = LoadR::fragment(sr, wr0, j, ks, lane);
+#pragma unroll
+        for (int j = 0; j < Cfg::TR; ++j)
+#pragma unroll
+          for (int i = 0; i < Cfg::TC; ++i) acc[j][i] = E::mma(fc[i], fr[j], acc[j][i]);
+      }
+      if (more) {
+        lr.put(lds + next);
+        lc.put(lds + next + LoadR::BYTES);
+      }
+      wait_direct();
+      __syncthreads();
+    }
+  }
+};
+
+// ---- results -------------------------------------------------------------------------------
+
+struct Result {
+  void* base;      // the tile's first element
+  int64_t ld;      // in elements
+  int rows, cols;  // of the tile that exist
+  int type;        // kFloat32, kBFloat16, kFloat16
+  int wide;        // 16-byte (16-bit: 8 values) stores are legal
+};
+
+__device__ __forceinline__ void store_value(void* base, int64_t at, int type, float v) {
+  if (type == kFloat32) static_cast<float*>(base)[at] = v;
+  else if (type == kBFloat16) static_cast<__bf16*>(base)[at] = (__bf16)v;
+  else static_cast<_Float16*>(base)[at] = (_Float16)v;
+}
+
+template <class Scalar>
+__device__ __forceinline__ void store_eight(void* base, int64_t at, const float (&v)[8]) {
+  Scalar out[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) out[q] = (Scalar)v[q];
+  constexpr int N = sizeof(out) / 16;
+  i32x4 piece[N];
+  __builtin_memcpy(piece, out, sizeof(out));
+#pragma unroll
+  for (int q = 0; q < N; ++q) reinterpret_cast<i32x4*>(static_cast<Scalar*>(base) + at)[q] = piece[q];
+}
+
+// scale: (row of tile, column of tile, accumulator) -> result.
+template <class Cfg, class Acc, class Scale>
+__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[Cfg::TR][Cfg::TC], const Scale& scale) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = lane & 15, g = lane >> 4;
+  const int wr0 = (wave % Cfg::WR) * (Cfg::TR * 16), wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
+#pragma unroll
+  for (int j = 0; j < Cfg::TR; ++j) {
+    const int r = wr0 + 16 * j + m;
+    if (r >= o.rows) continue;
+#pragma unroll
+    for (int i = 0; i < Cfg::TC; i += 2) {
+      const int c = wc0 + 32 * (i >> 1) + 8 * g;
+      if (c >= o.cols) continue;
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = scale(r, min(c + q, o.cols - 1), acc[j][i + (q >> 2)][q & 3]);
+      const int64_t at = (int64_t)r * o.ld + c;
+      if (o.wide && c + 8 <= o.cols) {
+        if (o.type == kFloat32) store_eight<float>(o.base, at, v);
+        else if (o.type == kBFloat16) store_eight<__bf16>(o.base, at, v);
+        else store_eight<_Float16>(o.base, at, v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (c + q < o.cols) store_value(o.base, at + q, o.type, v[q]);
+      }
+    }
+  }
+}
+
+struct Unscaled {
+  __device__ __forceinline__ float operator()(int, int, float v) const { return v; }
+};
+// The integer sum is exact; it is rounded to fp32 once, then scaled by the token and by the channel.
+struct TokenChannel {
+  const float* token;
+  const float* channel;
+  __device__ __forceinline__ float operator()(int r, int c, int v) const { return (float)v * token[r] * channel[c]; }
+};
+
+// ---- kernels -------------------------------------------------------------------------------
+
+struct RowProblem {
+  RowGroups groups;
+  const char* r;       // tokens x k
+  const char* c;       // experts x (columns x k, or k x columns)
+  int64_t ldr, ldc;    // bytes
+  int64_t stride_c;    // bytes from one expert's matrix to the next
+  int cols, k;
+  int tiles_c;
+  void* y;
+  int64_t ldy;         // elements
+  int out_type;
+  int wide;
+  const float* token_scale;    // 8-bit product only
+  const float* channel_scale;
+};
+
+__device__ __forceinline__ int type_bytes(int type) { return type == kFloat32 ? 4 : 2; }
+
+template <class E, Layout LC, Source S, class Cfg>
+__global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
+  using Product = TileProduct<E, KC, S, LC, S, Cfg>;
+  __shared__ __attribute__((aligned(1024))) char lds[Product::LDS_BYTES];
+  RowTile tile;
+  int tile_c;
+  if (!locate_rows<Cfg::BR>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
+  const int c0 = tile_c * Cfg::BC;
+  const bool rest = tile.expert >= p.groups.experts;
+  Operand r, c;
+  r.base = p.r + (int64_t)tile.row * p.ldr;
+  r.ld = p.ldr;
+  r.valid = tile.rows;
+  c.base = p.c + (int64_t)tile.expert * p.stride_c + (LC == KC ? (int64_t)c0 * p.ldc : (int64_t)c0 * E::SIZE);
+  c.ld = p.ldc;
+  c.valid = min(Cfg::BC, p.cols - c0);
+  r.exponents = c.exponents = nullptr;
+  r.ld_exp = c.ld_exp = 0;
+  typename E::Acc acc[Cfg::TR][Cfg::TC];
+  Product::run(r, c, rest ? 0 : p.k, lds, acc);
+  Result o;
+  o.base = static_cast<char*>(p.y) + ((int64_t)tile.row * p.ldy + c0) * type_bytes(p.out_type);
+  o.ld = p.ldy;
+  o.rows = tile.rows;
+  o.cols = c.valid;
+  o.type = p.out_type;
+  o.wide = p.wide;
+  if constexpr (E::SIZE == 1)
+    store_tile<Cfg>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0});
+  else
+    store_tile<Cfg>(o, acc, Unscaled{});
+}
+
+struct SumProblem {
+  RowGroups groups;
+  const char* r;          // tokens x rows
+  const char* c;          // tokens x cols (values, or codes)
+  int64_t ldr, ldc;       // bytes
+  const uint8_t* exponents;
+  int64_t ld_exp;
+  int rows, cols;
+  int tiles_r, tiles_c;
+  void* d;
+  int64_t ldd, stride_d;  // elements
+  int out_type;
+  int wide;
+};
+
+// Workgroup -> expert and tile of its matrix.  Experts differ in their rows, so each one's tiles are
+// spread over all XCDs, and each XCD has a contiguous part of them.
+__device__ __forceinline__ bool locate_sum(int wg, int experts, int tiles_r, int tiles_c, int& e, int& tr, int& tc) {
+  const int64_t tiles = (int64_t)tiles_r * tiles_c;
+  const int64_t chunk = (tiles + 7) >> 3;
+  const int64_t slot = wg >> 3;
+  e = (int)(slot / chunk);
+  const int64_t t = (wg & 7) * chunk + slot % chunk;
+  if (e >= experts || t >= tiles) return false;
+  constexpr int GR = 8;
+  const int64_t per = (int64_t)GR * tiles_c;
+  const int band = (int)(t / per), in_band = (int)(t - band * per);
+  const int rows = min(GR, tiles_r - band * GR);
+  tr = band * GR + in_band % rows;
+  tc = in_band / rows;
+  return true;
+}
+
+template <class E, Source SR, Source SC, class Cfg>
+__global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
+  using Product = TileProduct<E, XC, SR, XC, SC, Cfg>;
+  __shared__ __attribute__((aligned(1024))) char lds[Product::LDS_BYTES];
+  int e, tr, tc;
+  if (!locate_sum(blockIdx.x, p.groups.experts, p.tiles_r, p.tiles_c, e, tr, tc)) return;
+  int begin, end;
+  group_rows(p.groups, e, begin, end);
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
+  const int r0 = tr * Cfg::BR, c0 = tc * Cfg::BC;
+  Operand r, c;
+  r.base = p.r + (int64_t)begin * p.ldr + (int64_t)r0 * E::SIZE;
+  r.ld = p.ldr;
+  r.valid = min(Cfg::BR, p.rows - r0);
+  c.base = p.c + (int64_t)begin * p.ldc + (int64_t)c0 * (SC == Codes ? 1 : E::SIZE);
+  c.ld = p.ldc;
+  c.valid = min(Cfg::BC, p.cols - c0);
+  r.exponents = nullptr;
+  r.ld_exp = 0;
+  c.exponents = SC == Codes ? p.exponents + (int64_t)begin * p.ld_exp + c0 / 128 : nullptr;
+  c.ld_exp = p.ld_exp;
+  typename E::Acc acc[Cfg::TR][Cfg::TC];
+  Product::run(r, c, end - begin, lds, acc);
+  Result o;
+  o.base = static_cast<char*>(p.d) + ((int64_t)e * p.stride_d + (int64_t)r0 * p.ldd + c0) * type_bytes(p.out_type);
+  o.ld = p.ldd;
+  o.rows = r.valid;
+  o.cols = c.valid;
+  o.type = p.out_type;
+  o.wide = p.wide;
+  store_tile<Cfg>(o, acc, Unscaled{});
+}
+
+// ---- fp32 ----------------------------------------------------------------------------------
+// The fp32 matrix product of gemm.hpp, tile by tile.  A row-major result is the column-major transposed
+// one, so its M runs over the columns and its N over the rows here.
+
+template <class Cfg>
+__device__ __forceinline__ void f32_tile(const float* a, int64_t lda, int trans_a, const float* b, int64_t ldb, int trans_b,
+                                         int m, int n, int k, float* c, int64_t ldc, bool vec_a, bool vec_b, float* smem) {
+  GemmProblem<float> p;
+  p.A = a; p.B = b; p.lda = lda; p.ldb = ldb;
+  p.M = m; p.N = n; p.K = k;
+  p.transA = trans_a; p.transB = trans_b;
+  p.vecA = vec_a; p.vecB = vec_b;
+  p.tiles_m = p.tiles_n = p.num_tiles = 1;
+  p.lower = 0;
+  p.k_chunk = k > 0 ? k : 1;
+  p.ksel_b = nullptr;
+  EpiStore<float> store{c, ldc, 1.0f, 0.0f};
+  gemm_tile_body<float, Cfg, EpiStore<float>, -1>(p, store, 0, 0, smem);
+}
+
+template <class Cfg>
+__global__ __launch_bounds__(Cfg::NT) void row_product_f32_kernel(RowProblem p, int weights_k_contiguous, int vec_w, int vec_x) {
+  __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
+  RowTile tile;
+  int tile_c;
+  if (!locate_rows<Cfg::BN>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
+  const int c0 = tile_c * Cfg::BM;
+  const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
+  const float* w = reinterpret_cast<const float*>(p.c + (int64_t)tile.expert * p.stride_c) +
+                   (weights_k_contiguous ? (int64_t)c0 * ldc : (int64_t)c0);
+  const float* x = reinterpret_cast<const float*>(p.r) + (int64_t)tile.row * ldr;
+  float* y = static_cast<float*>(p.y) + (int64_t)tile.row * p.ldy + c0;
+  f32_tile<Cfg>(w, ldc, weights_k_contiguous, x, ldr, 0, min(Cfg::BM, p.cols - c0), tile.rows,
+                tile.expert >= p.groups.experts ? 0 : p.k, y, p.ldy, vec_w, vec_x, smem);
+}
+
+template <class Cfg>
+__global__ __launch_bounds__(Cfg::NT) void sum_product_f32_kernel(SumProblem p, int vec_dy, int vec_x) {
+  __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
+  int e, tr, tc;
+  if (!locate_sum(blockIdx.x, p.groups.experts, p.tiles_r, p.tiles_c, e, tr, tc)) return;
+  int begin, end;
+  group_rows(p.groups, e, begin, end);
+  const int r0 = tr * Cfg::BN, c0 = tc * Cfg::BM;
+  const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
+  const float* dy = reinterpret_cast<const float*>(p.r) + (int64_t)begin * ldr + r0;
+  const float* x = reinterpret_cast<const float*>(p.c) + (int64_t)begin * ldc + c0;
+  float* d = static_cast<float*>(p.d) + (int64_t)e * p.stride_d + (int64_t)r0 * p.ldd + c0;
+  f32_tile<Cfg>(x, ldc, 0, dy, ldr, 1, min(Cfg::BM, p.cols - c0), min(Cfg::BN, p.rows - r0), end - begin, d, p.ldd,
+                vec_x, vec_dy, smem);
+}
+
+// ---- 8-bit codes ---------------------------------------------------------------------------
+
+// Eight values of a row from column c on; behind the last column zeros.
+template <class T>
+__device__ __forceinline__ void load_eight(const T* row, int c, int cols, bool vec, float (&v)[8]) {
+  if (vec && c + 8 <= cols) {
+    constexpr int N = 8 * sizeof(T) / 16;
+    i32x4 piece[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) piece[i] = reinterpret_cast<const i32x4*>(row + c)[i];
+    T t[8];
+    __builtin_memcpy(t, piece, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? (float)row[c + i] : 0.0f;
+  }
+}
+
+__device__ __forceinline__ void store_codes(int8_t* row, int c, int cols, bool vec, const int (&q)[8]) {
+  if (vec && c + 8 <= cols) {
+    unsigned w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i >> 2] |= (unsigned)(q[i] & 255) << (8 * (i & 3));
+    *reinterpret_cast<uint2*>(row + c) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) row[c + i] = (int8_t)q[i];
+  }
+}
+
+// Largest magnitude so far, as the bits of its float: magnitudes compare like their bits as unsigned
+// numbers, and infinities and NaN compare above every finite one, so that one maximum finds both.
+__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+constexpr int kRowRegisters = 4;  // chunks of eight values that a thread keeps between the two passes
+
+// codes = round(127 x / top), scale = top / 127, with top the largest magnitude of the row.  A row of
+// zeros has scale 0; a row that holds an infinity or NaN has scale NaN and codes 0, so that everything
+// it stands for is NaN.  TPR threads take a row.
+template <class T, int TPR>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int rows, int cols, int vec_x,
+                                                            int8_t* codes, int64_t ldq, int vec_q, float* scales) {
+  constexpr int ROWS = 256 / TPR;
+  const int row = blockIdx.x * ROWS + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const bool mine = row < rows;
+  const T* in = x + (int64_t)(mine ? row : 0) * ldx;
+  const int chunks = mine ? (cols + 7) / 8 : 0;
+  float kept[kRowRegisters][8];
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < kRowRegisters; ++j) {
+    const int c = t + j * TPR;
+    if (c < chunks) {
+      load_eight(in, c * 8, cols, vec_x, kept[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, magnitude(kept[j][i]));
+    }
+  }
+  for (int c = t + kRowRegisters * TPR; c < chunks; c += TPR) {
+    float v[8];
+    load_eight(in, c * 8, cols, vec_x, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+  if constexpr (TPR > 64) {
+    __shared__ unsigned part[TPR / 64];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TPR / 64; ++w) top = max(top, part[w]);
+  }
+  if (!mine) return;
+  const bool finite = top < 0x7f800000u;
+  const float largest = __uint_as_float(top);
+  // Both the row and its maximum are brought to around 1 by a power of two, so that neither 127 x nor
+  // the reciprocal leaves the range.  127 x is exact for 16-bit inputs; one correction of the quotient
+  // by its remainder gives the correctly rounded one.
+  int power = 0;
+  const float b = frexpf(finite ? largest : 0.0f, &power);
+  const float inverse = b > 0.0f ? 1.0f / b : 0.0f;
+  if (t == 0) scales[row] = finite ? largest / 127.0f : __uint_as_float(0x7fc00000u);
+  int8_t* out = codes + (int64_t)row * ldq;
+  auto quantize = [&](const float (&v)[8], int c) {
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = 127.0f * ldexpf(v[i], -power);
+      float r = a * inverse;
+      r = __builtin_fmaf(__builtin_fmaf(-r, b, a), inverse, r);
+      q[i] = finite ? (int)__builtin_rintf(r) : 0;
+    }
+    store_codes(out, c * 8, cols, vec_q, q);
+  };
+#pragma unroll
+  for (int j = 0; j < kRowRegisters; ++j) {
+    const int c = t + j * TPR;
+    if (c < chunks) quantize(kept[j], c);
+  }
+  for (int c = t + kRowRegisters * TPR; c < chunks; c += TPR) {
+    float v[8];
+    load_eight(in, c * 8, cols, vec_x, v);
+    quantize(v, c);
+  }
+}
+
+constexpr int kCheckpointBlock = 128;  // columns that share an exponent
+
+// Activation checkpoints: with 2^(p-1) <= top < 2^p the largest magnitude of 128 columns of a row, the
+// step is 2^(p-7) (at least 2^-126; 2^-24, the smallest fp16 value, for fp16) and the codes are
+// round(x / step) held to -127..127; the exponent is stored with 127 added, 255 marks a block that holds
+// an infinity or NaN.  The step is a power of two because it stands inside the weight gradient's sum:
+// code * step and its product with a 16-bit gradient are then exact.  Sixteen lanes take a block.
+template <class T>
+__global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, int blocks,
+                                                         int vec_x, int8_t* codes, int64_t ldq, int vec_q,
+                                                         uint8_t* exponents, int64_t ld_exp, int lowest) {
+  const int64_t block = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+  const int64_t row = block / blocks;
+  if (row >= rows) return;  // (whole groups of 16 lanes leave)
+  const int in_row = (int)(block - row * blocks), t = threadIdx.x & 15;
+  const int c = in_row * kCheckpointBlock + t * 8;
+  float v[8];
+  load_eight(x + row * ldx, c, cols, vec_x, v);
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, d));
+  const bool finite = top < 0x7f800000u;
+  // exponent field of top, minus 6, is that of 2^(p-7); a subnormal top has field 0 and takes the lowest
+  const int code = max((int)(top >> 23) - 6, lowest);
+  const float per_step = __uint_as_float((unsigned)(254 - code) << 23);  // 2^(127 - code)
+  int q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = finite ? (int)fminf(fmaxf(__builtin_rintf(v[i] * per_step), -127.0f), 127.0f) : 0;
+  store_codes(codes + row * ldq, c, cols, vec_q, q);
+  if (t == 0) exponents[row * ld_exp + in_row] = (uint8_t)(finite ? code : 255);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void restore_kernel(const int8_t* codes, int64_t ldq, int vec_q, const uint8_t* exponents,
+                                                      int64_t ld_exp, int64_t rows, int cols, int pieces, T* x, int64_t ldx,
+                                                      int vec_x) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / pieces;
+  if (row >= rows) return;
+  const int c = (int)(at - row * pieces) * 8;
+  const int8_t* in = codes + row * ldq;
+  int8_t q[8];
+  if (vec_q && c + 8 <= cols) {
+    __builtin_memcpy(q, __builtin_assume_aligned(in + c, 8), 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = c + i < cols ? in[c + i] : 0;
+  }
+  const float step = exponent_value(exponents[row * ld_exp + c / kCheckpointBlock]);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)q[i] * step;
+  T* out = x + row * ldx;
+  if (vec_x && c + 8 <= cols) {
+    store_eight<T>(out, c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) out[c + i] = (T)v[i];
+  }
+}
+
+}  // namespace soapmi

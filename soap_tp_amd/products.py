@@ -1,0 +1,444 @@
+"""Products of the layers whose weights SOAP trains: grouped by expert, from 8-bit activation
+checkpoints, and in 8-bit integers.
+
+The reference starts from a gradient matrix.  These are the products of a layer's forward and
+backward pass up to that matrix, on the same library (``include/soap_mi355.h``) and in the same
+manner as ``soap_tp_amd.ops``: device tensors only, work is enqueued on torch's current stream of the
+tensors' device and never synchronised, bad arguments raise ``ValueError`` before anything is launched.
+
+Tokens are rows.  With experts, the rows are sorted by expert and ``ends`` (int64, on the device) holds
+for each expert the first row behind its own: expert ``e`` has the rows ``ends[e-1] .. ends[e]-1``.  An
+expert may have no row, and the buffer may have rows behind the last expert's.  The sizes stay on the
+device, so nothing here depends on their values on the host and calls can be captured into a graph.
+Weights are (outputs, inputs) matrices, ``(experts, outputs, inputs)`` with experts; a dense layer
+passes ``ends=None`` and two-dimensional weights.  Inputs are bfloat16, float16 or float32, rows may be
+strided, sums are formed in float32 on the matrix cores.
+
+    y  = expert_product(x, weights, ends)                   # y[t] = W_e x[t]
+    dx = expert_input_gradient(dy, weights, ends)           # dx[t] = W_e^T dy[t]
+    dw = expert_weight_gradient(dy, x, ends)                # dW_e = sum of dy[t] x[t]^T, float32
+    update = soap_step(dw[e], state[e], ...)
+
+``expert_linear`` is the first of them for autograd, with the other two as its backward pass.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from .ops._common import native_call, require_device_tensor, stream_of
+
+__all__ = [
+    "ActivationCheckpoint",
+    "checkpoint_activations",
+    "expert_input_gradient",
+    "expert_linear",
+    "expert_product",
+    "expert_weight_gradient",
+    "int8_product",
+    "quantize_tokens",
+    "restore_activations",
+]
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+CHECKPOINT_BLOCK = 128  # columns that share an exponent
+_INT8_MAX_INNER = 131071  # 16384 times more of them would leave 32-bit sums
+
+
+class ActivationCheckpoint(NamedTuple):
+    """A matrix kept in 8 bits: ``codes`` (int8, its shape) and ``exponents`` (uint8, one for each row
+    and 128 columns); the values are ``codes * 2 ** (exponents - 127)``, NaN where the exponent is 255.
+    ``dtype`` is the type of the matrix it was made from."""
+
+    codes: Tensor
+    exponents: Tensor
+    dtype: torch.dtype
+
+
+# ---- checks --------------------------------------------------------------------------------
+
+
+def _check_matrix(name: str, tensor: Tensor, dimensions: int = 2) -> None:
+    if not isinstance(tensor, Tensor):
+        raise ValueError(f"{name} must be a tensor, got {type(tensor).__name__}.")
+    if tensor.ndim != dimensions:
+        raise ValueError(f"{name} must be {dimensions}D, got {tensor.ndim}D.")
+
+
+def _check_values(name: str, tensor: Tensor, dimensions: int = 2) -> None:
+    _check_matrix(name, tensor, dimensions)
+    if tensor.dtype not in _DTYPES:
+        raise ValueError(f"{name} must use float32, bfloat16 or float16, got {tensor.dtype}.")
+
+
+def _check_together(device: torch.device, **tensors: Tensor) -> None:
+    for name, tensor in tensors.items():
+        if tensor.device != device:
+            raise ValueError(f"{name} is on {tensor.device}, expected {device}.")
+        require_device_tensor(name, tensor)
+
+
+def _rows(tensor: Tensor) -> Tuple[Tensor, int]:
+    """The tensor with its last dimension contiguous (copied if it is not) and its row stride."""
+    columns = tensor.size(-1)
+    stride = tensor.stride(-2) if tensor.size(-2) > 1 else max(1, columns)
+    if (columns > 1 and tensor.stride(-1) != 1) or stride < max(1, columns):
+        tensor = tensor.contiguous()
+        stride = max(1, columns)
+    return tensor, stride
+
+
+def _experts(tensor: Tensor) -> Tuple[Tensor, int, int]:
+    """Weights as (tensor, row stride, expert stride)."""
+    tensor, row = _rows(tensor)
+    if tensor.ndim == 2:
+        return tensor, row, 0
+    if tensor.size(0) > 1 and tensor.stride(0) < 0:
+        tensor = tensor.contiguous()
+        row = max(1, tensor.size(-1))
+    return tensor, row, tensor.stride(0) if tensor.size(0) > 1 else 0
+
+
+def _check_ends(ends: Optional[Tensor], experts: int) -> int:
+    if ends is None:
+        return 0
+    _check_matrix("ends", ends, 1)
+    if ends.dtype != torch.int64:
+        raise ValueError(f"ends must use int64, got {ends.dtype}.")
+    if ends.numel() != experts:
+        raise ValueError(f"ends has {ends.numel()} entries, expected one for each of {experts} experts.")
+    if ends.numel() > 1 and ends.stride(0) != 1:
+        raise ValueError("ends must be contiguous.")
+    return ends.data_ptr()
+
+
+def _spans(tensor: Tensor) -> Tuple[int, int]:
+    """First and last byte of memory that a tensor's elements use."""
+    first = tensor.data_ptr()
+    reach = sum((size - 1) * abs(stride) for size, stride in zip(tensor.shape, tensor.stride()))
+    return first, first + (reach + 1) * tensor.element_size()
+
+
+def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, ...], **inputs: Tensor) -> None:
+    """``out`` as a caller gave it: rows of contiguous values, written in place, apart from the inputs."""
+    _check_matrix("out", out, len(shape))
+    if tuple(out.shape) != shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, expected {shape}.")
+    if out.dtype not in dtypes:
+        raise ValueError(f"out must use {' or '.join(str(d) for d in dtypes)}, got {out.dtype}.")
+    if out.numel() == 0:
+        return
+    if (shape[-1] > 1 and out.stride(-1) != 1) or (shape[-2] > 1 and out.stride(-2) < shape[-1]):
+        raise ValueError("out must have contiguous rows that do not overlap.")
+    if len(shape) == 3 and shape[0] > 1 and out.stride(0) < (shape[1] - 1) * out.stride(1) + shape[2]:
+        raise ValueError("out must have matrices that do not overlap.")
+    first, last = _spans(out)
+    for name, tensor in inputs.items():
+        if tensor is not None and tensor.numel():
+            low, high = _spans(tensor)
+            if low < last and first < high:
+                raise ValueError(f"out must not overlap {name}.")
+
+
+def _row_stride(tensor: Tensor) -> int:
+    return tensor.stride(-2) if tensor.size(-2) > 1 else max(1, tensor.size(-1))
+
+
+def _out_types(dtype: torch.dtype) -> Tuple[torch.dtype, ...]:
+    return (dtype,) if dtype == torch.float32 else (dtype, torch.float32)
+
+
+# ---- grouped products ----------------------------------------------------------------------
+
+
+def _grouped(x: Tensor, weights: Tensor, ends: Optional[Tensor], out: Optional[Tensor], transposed: bool, name: str) -> Tensor:
+    _check_values(name, x)
+    _check_values("weights", weights, 2 if ends is None else 3)
+    if weights.dtype != x.dtype:
+        raise ValueError(f"weights must use {x.dtype} as {name} does, got {weights.dtype}.")
+    outputs, inputs = weights.shape[-2:]
+    inner, columns = (outputs, inputs) if transposed else (inputs, outputs)
+    if x.size(1) != inner:
+        raise ValueError(f"{name} has {x.size(1)} columns, expected {inner}.")
+    experts = 1 if ends is None else weights.size(0)
+    pointer = _check_ends(ends, experts)
+    tokens = x.size(0)
+    tensors = {name: x, "weights": weights, **({} if ends is None else {"ends": ends})}
+    if out is not None:
+        _check_out(out, (tokens, columns), _out_types(x.dtype), **tensors)
+        tensors["out"] = out
+    _check_together(x.device, **tensors)
+    fresh = out is None
+    if fresh:
+        out = torch.empty((tokens, columns), dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    with torch.cuda.device(x.device):
+        rows, ldx = _rows(x)
+        matrices, ldw, stride_w = _experts(weights)
+        native_call(
+            "soapmi_expert_product", _DTYPES[x.dtype], rows.data_ptr(), ldx, matrices.data_ptr(), ldw, stride_w,
+            1 if transposed else 0, pointer, experts, tokens, outputs, inputs, _DTYPES[out.dtype], out.data_ptr(),
+            _row_stride(out), 1 if fresh else 0, stream_of(x),
+        )
+    return out
+
+
+@torch.no_grad()
+def expert_product(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, out: Optional[Tensor] = None) -> Tensor:
+    """``y[t] = W_e x[t]`` for every row ``t`` of every expert ``e``.
+
+    ``x`` is (tokens, inputs), ``weights`` (experts, outputs, inputs) of the same type; the result is
+    (tokens, outputs) of that type.  ``out`` receives the result instead of a new tensor and may be
+    float32.  Rows of no expert are zero in a new tensor and left as they were in ``out``."""
+    return _grouped(x, weights, ends, out, False, "x")
+
+
+@torch.no_grad()
+def expert_input_gradient(gradient: Tensor, weights: Tensor, ends: Optional[Tensor], *, out: Optional[Tensor] = None) -> Tensor:
+    """``dx[t] = W_e^T dy[t]``: the gradient of ``expert_product``'s ``x`` from that of its result,
+    (tokens, inputs) from (tokens, outputs); otherwise as ``expert_product``."""
+    return _grouped(gradient, weights, ends, out, True, "gradient")
+
+
+@torch.no_grad()
+def expert_weight_gradient(
+    gradient: Tensor,
+    x: Union[Tensor, ActivationCheckpoint],
+    ends: Optional[Tensor],
+    *,
+    out: Optional[Tensor] = None,
+    out_dtype: torch.dtype = torch.float32,
+) -> Tensor:
+    """``dW_e = sum over e's rows t of dy[t] x[t]^T``: (experts, outputs, inputs), or (outputs, inputs)
+    without ``ends``; zeros for an expert without rows.
+
+    ``gradient`` is (tokens, outputs); ``x`` (tokens, inputs) of the same type, or the checkpoint that
+    was made from it.  The result is float32, the type ``soap_step`` takes, or ``out_dtype`` (the
+    gradient's own type); ``out`` receives it instead of a new tensor."""
+    _check_values("gradient", gradient)
+    saved = isinstance(x, ActivationCheckpoint)
+    if saved:
+        _check_checkpoint(x)
+        tokens, inputs, dtype = x.codes.size(0), x.codes.size(1), x.dtype
+    else:
+        _check_values("x", x)
+        tokens, inputs, dtype = x.size(0), x.size(1), x.dtype
+    if dtype != gradient.dtype:
+        raise ValueError(f"x must use {gradient.dtype} as gradient does, got {dtype}.")
+    if gradient.size(0) != tokens:
+        raise ValueError(f"gradient has {gradient.size(0)} rows, expected {tokens}.")
+    outputs = gradient.size(1)
+    if ends is not None:
+        _check_matrix("ends", ends, 1)
+    experts = 1 if ends is None else ends.numel()
+    pointer = _check_ends(ends, experts)
+    shape = (outputs, inputs) if ends is None else (experts, outputs, inputs)
+    parts = {"codes": x.codes, "exponents": x.exponents} if saved else {"x": x}
+    tensors = {"gradient": gradient, **parts, **({} if ends is None else {"ends": ends})}
+    if out is not None:
+        _check_out(out, shape, _out_types(dtype), **tensors)
+        tensors["out"] = out
+    elif out_dtype not in _out_types(dtype):
+        raise ValueError(f"out_dtype must be {' or '.join(str(d) for d in _out_types(dtype))}, got {out_dtype}.")
+    _check_together(gradient.device, **tensors)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype, device=gradient.device)
+    if out.numel() == 0:
+        return out
+    if saved and dtype == torch.float32:
+        x, saved = restore_activations(x), False  # the matrix cores take no 8-bit values beside fp32
+    stride = out.stride(0) if out.ndim == 3 and experts > 1 else 0
+    with torch.cuda.device(gradient.device):
+        rows, ldg = _rows(gradient)
+        tail = (pointer, experts, tokens, outputs, inputs, _DTYPES[out.dtype], out.data_ptr(), _row_stride(out), stride,
+                stream_of(gradient))
+        if saved:
+            native_call("soapmi_expert_weight_gradient_saved", _DTYPES[dtype], rows.data_ptr(), ldg, x.codes.data_ptr(),
+                        _row_stride(x.codes), x.exponents.data_ptr(), _row_stride(x.exponents), *tail)
+        else:
+            values, ldx = _rows(x)
+            native_call("soapmi_expert_weight_gradient", _DTYPES[dtype], rows.data_ptr(), ldg, values.data_ptr(), ldx, *tail)
+    return out
+
+
+class _ExpertLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, ends, checkpoint):
+        y = expert_product(x, weights, ends)
+        kept = x
+        if ctx.needs_input_grad[1] and checkpoint:
+            kept = checkpoint_activations(x)
+        ctx.dtype = x.dtype
+        if isinstance(kept, ActivationCheckpoint):
+            ctx.save_for_backward(weights, ends, kept.codes, kept.exponents)
+        else:
+            ctx.save_for_backward(weights, ends, x if ctx.needs_input_grad[1] else None, None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gradient):
+        weights, ends, kept, exponents = ctx.saved_tensors
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = expert_input_gradient(gradient, weights, ends)
+        if ctx.needs_input_grad[1]:
+            x = kept if exponents is None else ActivationCheckpoint(kept, exponents, ctx.dtype)
+            dw = expert_weight_gradient(gradient, x, ends, out_dtype=weights.dtype)
+        return dx, dw, None, None
+
+
+def expert_linear(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, checkpoint: bool = False) -> Tensor:
+    """``expert_product`` for autograd: gradients of ``x`` and ``weights`` come from
+    ``expert_input_gradient`` and ``expert_weight_gradient``.
+
+    With ``checkpoint`` the input is kept for the backward pass in 8 bits (``checkpoint_activations``)
+    instead of in its own type; the weights' gradient is then that of the restored input, ``x``'s
+    gradient and the result are unchanged."""
+    return _ExpertLinear.apply(x, weights, ends, checkpoint)
+
+
+# ---- activation checkpoints ----------------------------------------------------------------
+
+
+def _check_checkpoint(checkpoint: ActivationCheckpoint) -> None:
+    if not isinstance(checkpoint, ActivationCheckpoint):
+        raise ValueError(f"checkpoint must be an ActivationCheckpoint, got {type(checkpoint).__name__}.")
+    _check_matrix("codes", checkpoint.codes)
+    _check_matrix("exponents", checkpoint.exponents)
+    if checkpoint.codes.dtype != torch.int8 or checkpoint.exponents.dtype != torch.uint8:
+        raise ValueError(f"codes and exponents must use int8 and uint8, got {checkpoint.codes.dtype} and "
+                         f"{checkpoint.exponents.dtype}.")
+    if checkpoint.dtype not in _DTYPES:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, got {checkpoint.dtype}.")
+    rows, columns = checkpoint.codes.shape
+    blocks = -(-columns // CHECKPOINT_BLOCK)
+    if tuple(checkpoint.exponents.shape) != (rows, blocks):
+        raise ValueError(f"exponents has shape {tuple(checkpoint.exponents.shape)}, expected {(rows, blocks)}.")
+    for name, tensor in (("codes", checkpoint.codes), ("exponents", checkpoint.exponents)):
+        size = tensor.size(1)
+        if tensor.numel() and ((size > 1 and tensor.stride(1) != 1) or (rows > 1 and tensor.stride(0) < size)):
+            raise ValueError(f"{name} must have contiguous rows.")
+
+
+def _code_matrix(rows: int, columns: int, device) -> Tensor:
+    """int8 rows that start at multiples of 16 bytes."""
+    return torch.empty((rows, -(-columns // 16) * 16), dtype=torch.int8, device=device)[:, :columns]
+
+
+@torch.no_grad()
+def checkpoint_activations(x: Tensor) -> ActivationCheckpoint:
+    """Keep a matrix in 8 bits, with a power-of-two step for each row and 128 columns: half the memory
+    of 16-bit activations.  A value is restored to within half a step (within a step above 127.5
+    steps), a step being at most 1/64 of the largest magnitude of its 128 columns."""
+    _check_values("x", x)
+    require_device_tensor("x", x)
+    rows, columns = x.shape
+    codes = _code_matrix(rows, columns, x.device)
+    exponents = torch.empty((rows, -(-columns // CHECKPOINT_BLOCK)), dtype=torch.uint8, device=x.device)
+    if x.numel():
+        with torch.cuda.device(x.device):
+            values, ldx = _rows(x)
+            native_call("soapmi_checkpoint_activations", _DTYPES[x.dtype], values.data_ptr(), ldx, rows, columns,
+                        codes.data_ptr(), _row_stride(codes), exponents.data_ptr(), _row_stride(exponents), stream_of(x))
+    return ActivationCheckpoint(codes, exponents, x.dtype)
+
+
+@torch.no_grad()
+def restore_activations(checkpoint: ActivationCheckpoint, *, out: Optional[Tensor] = None) -> Tensor:
+    """The matrix that a checkpoint stands for, in the type it was made from."""
+    _check_checkpoint(checkpoint)
+    codes, exponents, dtype = checkpoint
+    rows, columns = codes.shape
+    tensors = {"codes": codes, "exponents": exponents}
+    if out is not None:
+        _check_out(out, (rows, columns), (dtype,), **tensors)
+        tensors["out"] = out
+    _check_together(codes.device, **tensors)
+    if out is None:
+        out = torch.empty((rows, columns), dtype=dtype, device=codes.device)
+    if out.numel():
+        with torch.cuda.device(codes.device):
+            native_call("soapmi_restore_activations", _DTYPES[dtype], codes.data_ptr(), _row_stride(codes),
+                        exponents.data_ptr(), _row_stride(exponents), rows, columns, out.data_ptr(), _row_stride(out),
+                        stream_of(codes))
+    return out
+
+
+# ---- 8-bit integer product -----------------------------------------------------------------
+
+
+@torch.no_grad()
+def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """Codes (int8) and scales (float32, one for each row) of a matrix: scale = largest magnitude / 127,
+    code = x / scale rounded to the nearest even.  The rows are tokens, or a weight's output channels.
+    A row of zeros has scale 0; one that holds an infinity or NaN has scale NaN."""
+    _check_values("x", x)
+    require_device_tensor("x", x)
+    rows, columns = x.shape
+    codes = _code_matrix(rows, columns, x.device)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if rows:
+        with torch.cuda.device(x.device):
+            values, ldx = _rows(x)
+            native_call("soapmi_quantize_rows", _DTYPES[x.dtype], values.data_ptr(), ldx, rows, columns, codes.data_ptr(),
+                        _row_stride(codes), scales.data_ptr(), stream_of(x))
+    return codes, scales
+
+
+def _check_codes(name: str, codes: Tensor, scales: Tensor) -> None:
+    _check_matrix(name, codes)
+    if codes.dtype != torch.int8:
+        raise ValueError(f"{name} must use int8, got {codes.dtype}.")
+    _check_matrix(f"{name}' scales", scales, 1)
+    if scales.dtype != torch.float32:
+        raise ValueError(f"{name}' scales must use float32, got {scales.dtype}.")
+    if scales.numel() != codes.size(0):
+        raise ValueError(f"{name} have {codes.size(0)} rows and {scales.numel()} scales.")
+    if scales.numel() > 1 and scales.stride(0) != 1:
+        raise ValueError(f"{name}' scales must be contiguous.")
+
+
+@torch.no_grad()
+def int8_product(
+    codes: Tensor,
+    scales: Tensor,
+    weight_codes: Tensor,
+    weight_scales: Tensor,
+    *,
+    out: Optional[Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+) -> Tensor:
+    """``y[t, j] = scales[t] weight_scales[j] sum over i of codes[t, i] weight_codes[j, i]``.
+
+    ``codes`` is (tokens, inputs), ``weight_codes`` (outputs, inputs), both as ``quantize_tokens`` makes
+    them from the rows of an activation and of a weight matrix; the integer sum is exact.  The result is
+    (tokens, outputs) of ``out_dtype`` (bfloat16, float16 or float32), or goes to ``out``."""
+    _check_codes("codes", codes, scales)
+    _check_codes("weight_codes", weight_codes, weight_scales)
+    tokens, inner = codes.shape
+    outputs = weight_codes.size(0)
+    if weight_codes.size(1) != inner:
+        raise ValueError(f"weight_codes have {weight_codes.size(1)} columns, expected {inner}.")
+    if inner > _INT8_MAX_INNER:
+        raise ValueError(f"codes have {inner} columns, at most {_INT8_MAX_INNER} keep the integer sums inside 32 bits.")
+    tensors = {"codes": codes, "scales": scales, "weight_codes": weight_codes, "weight_scales": weight_scales}
+    if out is not None:
+        _check_out(out, (tokens, outputs), tuple(_DTYPES), **tensors)
+        tensors["out"] = out
+    elif out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}.")
+    _check_together(codes.device, **tensors)
+    if out is None:
+        out = torch.empty((tokens, outputs), dtype=out_dtype, device=codes.device)
+    if out.numel():
+        with torch.cuda.device(codes.device):
+            rows, ldq = _rows(codes)
+            matrix, ldw = _rows(weight_codes)
+            native_call("soapmi_int8_product", rows.data_ptr(), ldq, scales.data_ptr(), matrix.data_ptr(), ldw,
+                        weight_scales.data_ptr(), tokens, outputs, inner, _DTYPES[out.dtype], out.data_ptr(),
+                        _row_stride(out), stream_of(codes))
+    return out

@@ -1,0 +1,161 @@
+"""Host-side checks of ``soap_tp_amd.products`` that need no GPU: every refusal is raised before
+anything is launched, by the Python layer and by the C entry points."""
+import pytest
+import torch
+
+import soap_tp_amd
+from soap_tp_amd import _native, products
+
+P = 4096  # a non-null address that no refused call dereferences
+
+
+def _ends(*values):
+    return torch.tensor(values, dtype=torch.int64)
+
+
+def test_products_are_public():
+    assert soap_tp_amd.products is products
+    assert sorted(products.__all__) == [
+        "ActivationCheckpoint", "checkpoint_activations", "expert_input_gradient", "expert_linear", "expert_product",
+        "expert_weight_gradient", "int8_product", "quantize_tokens", "restore_activations"]
+    for name in products.__all__:
+        assert getattr(products, name).__doc__
+
+
+X, W, DY = torch.zeros(6, 8), torch.zeros(2, 4, 8), torch.zeros(6, 4)
+
+
+@pytest.mark.parametrize("arguments,message", [
+    (dict(x=torch.zeros(8)), "x must be 2D"),
+    (dict(x=[1.0]), "x must be a tensor"),
+    (dict(x=X.double()), "x must use float32, bfloat16 or float16"),
+    (dict(weights=torch.zeros(4, 8)), "weights must be 3D"),
+    (dict(ends=None), "weights must be 2D"),
+    (dict(weights=W.half()), "weights must use torch.float32"),
+    (dict(x=torch.zeros(6, 7)), "x has 7 columns, expected 8"),
+    (dict(ends=_ends(1, 2, 3)), "ends has 3 entries"),
+    (dict(ends=_ends(3, 6).int()), "ends must use int64"),
+    (dict(ends=_ends(3, 0, 6, 0)[::2]), "ends must be contiguous"),
+    (dict(ends=_ends(3, 6).view(1, 2)), "ends must be 1D"),
+    (dict(out=torch.zeros(6, 5)), "out has shape"),
+    (dict(out=torch.zeros(6, 4).half()), "out must use torch.float32"),
+    (dict(out=torch.zeros(4, 6).T), "out must have contiguous rows"),
+    (dict(out=torch.zeros(1, 4).expand(6, 4)), "out must have contiguous rows"),
+    (dict(out=X[:, 1:5]), "out must not overlap x"),
+    (dict(out=W.view(-1)[:24].view(6, 4)), "out must not overlap weights"),
+    (dict(), "requires cuda buffers"),
+])
+def test_expert_product_refusals(arguments, message):
+    call = dict(x=X, weights=W, ends=_ends(3, 6), **{"out": None})
+    call.update(arguments)
+    with pytest.raises(ValueError, match=message):
+        products.expert_product(call["x"], call["weights"], call["ends"], out=call["out"])
+
+
+def test_input_gradient_refusals():
+    with pytest.raises(ValueError, match="gradient has 8 columns, expected 4"):
+        products.expert_input_gradient(X, W, _ends(3, 6))
+    with pytest.raises(ValueError, match="requires cuda buffers"):
+        products.expert_input_gradient(DY, W, _ends(3, 6))
+    with pytest.raises(ValueError, match="requires cuda buffers"):
+        products.expert_linear(X, W, _ends(3, 6))
+
+
+def _saved(rows=6, columns=8, dtype=torch.float32):
+    return products.ActivationCheckpoint(torch.zeros(rows, columns, dtype=torch.int8),
+                                         torch.zeros(rows, -(-columns // 128), dtype=torch.uint8), dtype)
+
+
+@pytest.mark.parametrize("arguments,message", [
+    (dict(gradient=torch.zeros(5, 4)), "gradient has 5 rows, expected 6"),
+    (dict(gradient=DY.half()), "x must use torch.float16"),
+    (dict(x=_saved(dtype=torch.bfloat16)), "x must use torch.float32"),
+    (dict(x=_saved(rows=5)), "gradient has 6 rows, expected 5"),
+    (dict(x=_saved()._replace(exponents=torch.zeros(6, 2, dtype=torch.uint8))), "exponents has shape"),
+    (dict(x=_saved()._replace(codes=torch.zeros(6, 8))), "codes and exponents must use int8 and uint8"),
+    (dict(x=_saved()._replace(codes=torch.zeros(8, 6, dtype=torch.int8).T)), "codes must have contiguous rows"),
+    (dict(x=_saved()._replace(dtype=torch.float64)), "dtype must be float32"),
+    (dict(ends=_ends(3, 6).int()), "ends must use int64"),
+    (dict(out_dtype=torch.bfloat16), "out_dtype must be torch.float32"),
+    (dict(out=torch.zeros(4, 8)), "out must be 3D"),
+    (dict(out=torch.zeros(4, 8).expand(2, 4, 8)), "matrices that do not overlap"),
+    (dict(x=_saved()), "requires cuda buffers"),
+    (dict(), "requires cuda buffers"),
+])
+def test_weight_gradient_refusals(arguments, message):
+    call = dict(gradient=DY, x=X, ends=_ends(3, 6))
+    call.update(arguments)
+    with pytest.raises(ValueError, match=message):
+        products.expert_weight_gradient(**call)
+
+
+def test_checkpoint_and_int8_refusals():
+    with pytest.raises(ValueError, match="requires cuda buffers"):
+        products.checkpoint_activations(X)
+    with pytest.raises(ValueError, match="x must use float32"):
+        products.checkpoint_activations(X.int())
+    with pytest.raises(ValueError, match="checkpoint must be an ActivationCheckpoint"):
+        products.restore_activations(X)
+    with pytest.raises(ValueError, match="out must use torch.float32"):
+        products.restore_activations(_saved(), out=X.half())
+    with pytest.raises(ValueError, match="requires cuda buffers"):
+        products.restore_activations(_saved())
+    with pytest.raises(ValueError, match="requires cuda buffers"):
+        products.quantize_tokens(X)
+    codes, scales = torch.zeros(6, 8, dtype=torch.int8), torch.zeros(6)
+    weights, channels = torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)
+    for arguments, message in (
+        ((codes.float(), scales, weights, channels), "codes must use int8"),
+        ((codes, scales[:5], weights, channels), "6 rows and 5 scales"),
+        ((codes, scales.double(), weights, channels), "scales must use float32"),
+        ((codes, torch.zeros(12)[::2], weights, channels), "scales must be contiguous"),
+        ((codes, scales, weights[:, :7], channels), "weight_codes have 7 columns, expected 8"),
+        ((codes, scales, weights, channels), "requires cuda buffers"),
+    ):
+        with pytest.raises(ValueError, match=message):
+            products.int8_product(*arguments)
+    with pytest.raises(ValueError, match="out_dtype must be float32"):
+        products.int8_product(codes, scales, weights, channels, out_dtype=torch.float64)
+    long = torch.zeros(1, 131072, dtype=torch.int8)
+    with pytest.raises(ValueError, match="131072 columns, at most 131071"):
+        products.int8_product(long, torch.zeros(1), long, torch.zeros(1))
+
+
+@pytest.mark.parametrize("name,arguments,message", [
+    ("soapmi_expert_product", (3, P, 8, P, 8, 32, 0, P, 2, 6, 4, 8, 3, P, 4, 0, None), "dtype must be 0"),
+    ("soapmi_expert_product", (1, P, 8, P, 8, 32, 0, P, 2, 6, 4, 8, 2, P, 4, 0, None), "out_dtype must be dtype or 0"),
+    ("soapmi_expert_product", (0, P, 8, P, 8, 32, 0, P, 2, -1, 4, 8, 0, P, 4, 0, None), "non-negative"),
+    ("soapmi_expert_product", (0, P, 8, P, 8, 32, 0, P, 2, 1 << 30, 4, 8, 0, P, 4, 0, None), "below 2\\^30"),
+    ("soapmi_expert_product", (0, P, 8, P, 8, 32, 0, None, 2, 6, 4, 8, 0, P, 4, 0, None), "ends may be null"),
+    ("soapmi_expert_product", (0, P, 7, P, 8, 32, 0, P, 2, 6, 4, 8, 0, P, 4, 0, None), "leading dimensions"),
+    ("soapmi_expert_product", (0, P, 4, P, 8, 32, 1, P, 2, 6, 4, 8, 0, P, 4, 0, None), "leading dimensions"),
+    ("soapmi_expert_product", (0, P, 8, P, 8, -1, 0, P, 2, 6, 4, 8, 0, P, 4, 0, None), "stride_w must be"),
+    ("soapmi_expert_product", (0, P, 8, None, 8, 32, 0, P, 2, 6, 4, 8, 0, P, 4, 0, None), "nonzero"),
+    ("soapmi_expert_weight_gradient", (0, P, 4, P, 8, P, 2, 6, 4, 8, 0, P, 8, 31, None), "must not overlap"),
+    ("soapmi_expert_weight_gradient", (0, P, 3, P, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None), "leading dimensions"),
+    ("soapmi_expert_weight_gradient", (0, P, 4, None, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None), "nonzero"),
+    ("soapmi_expert_weight_gradient_saved", (0, P, 4, P, 8, P, 1, P, 2, 6, 4, 8, 0, P, 8, 32, None), "restore a float32"),
+    ("soapmi_expert_weight_gradient_saved", (1, P, 4, P, 8, P, 0, P, 2, 6, 4, 8, 0, P, 8, 32, None), "leading dimensions"),
+    ("soapmi_checkpoint_activations", (0, P, 8, 6, 8, P, 8, P, 0, None), "leading dimensions"),
+    ("soapmi_checkpoint_activations", (0, None, 8, 6, 8, P, 8, P, 1, None), "nonzero"),
+    ("soapmi_restore_activations", (7, P, 8, P, 1, 6, 8, P, 8, None), "dtype must be 0"),
+    ("soapmi_quantize_rows", (0, P, 8, 6, 8, P, 7, P, None), "leading dimensions"),
+    ("soapmi_int8_product", (P, 131072, P, P, 131072, P, 6, 4, 131072, 1, P, 4, None), "at most 131071"),
+    ("soapmi_int8_product", (P, 8, None, P, 8, P, 6, 4, 8, 1, P, 4, None), "nonzero"),
+])
+def test_entry_points_refuse(name, arguments, message):
+    with pytest.raises(ValueError, match=message):
+        _native.call(name, *arguments)
+
+
+@pytest.mark.parametrize("name,arguments", [
+    ("soapmi_expert_product", (1, None, 8, None, 8, 32, 0, P, 0, 0, 4, 8, 1, None, 4, 1, None)),
+    ("soapmi_expert_product", (1, None, 8, None, 8, 0, 0, None, 1, 6, 0, 8, 1, None, 0, 1, None)),
+    ("soapmi_expert_weight_gradient", (1, None, 4, None, 0, None, 1, 6, 4, 0, 1, None, 0, 0, None)),
+    ("soapmi_checkpoint_activations", (1, None, 8, 0, 8, None, 8, None, 1, None)),
+    ("soapmi_restore_activations", (1, None, 0, None, 0, 0, 0, None, 0, None)),
+    ("soapmi_quantize_rows", (1, None, 8, 0, 8, None, 8, None, None)),
+    ("soapmi_int8_product", (None, 8, None, None, 8, None, 0, 4, 8, 1, None, 4, None)),
+])
+def test_empty_results_need_no_buffers(name, arguments):
+    _native.call(name, *arguments)
