@@ -186,27 +186,36 @@ struct Operand {
 constexpr unsigned kOutside = 0xC0000000u;    // a byte offset outside every buffer: such a lane fetches zeros
 constexpr int kBufferBytes = 0x40000000;
 
-// 16 bytes per lane from memory to LDS at lds + 16 * lane (lds: the same in all lanes of a wavefront).
+// 16 bytes per lane from memory (resource's address + offset + more) to LDS at lds + 16 * lane (more and lds:
+// the same in all lanes of a wavefront); zeros where the resource ends before them.
 // In inline assembly because the compiler, told of such a load, waits for it before every transposing
 // LDS read, the ones of the other buffer included.  There is no output register; the waits are
-// wait_direct().
-__device__ __forceinline__ void load_to_lds(i32x4 resource, unsigned offset, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+// wait_arrived().
+__device__ __forceinline__ void load_to_lds(i32x4 resource, unsigned offset, unsigned more, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(lds), "v"(offset), "s"(resource)
+               : "s"(lds), "v"(offset), "s"(resource), "s"(more)
                : "memory", "m0");
 }
-__device__ __forceinline__ void wait_direct() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Every load to LDS and every LDS access that this wavefront has started is done, and so is every other
+// wavefront's of the workgroup.
+__device__ __forceinline__ void wait_arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-__device__ __forceinline__ i32x4 buffer_of(const char* base) {
+__device__ __forceinline__ i32x4 buffer_of(const char* base, int bytes) {
   const uint64_t address = reinterpret_cast<uint64_t>(base);
   i32x4 r;
   r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)address);
   r[1] = __builtin_amdgcn_readfirstlane((int)((address >> 32) & 0xffff));
-  r[2] = kBufferBytes;
+  r[2] = __builtin_amdgcn_readfirstlane(bytes);
   r[3] = 0x00020000;
   return r;
 }
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // all but the last N loads of this wavefront are done
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 __device__ __forceinline__ i32x4 load_bytes(const char* p, int count) {
   i32x4 v = {0, 0, 0, 0};
@@ -237,14 +246,22 @@ struct Loader {
   static_assert(S != Direct || PIECES % 64 == 0, "whole wavefronts fetch");
   static constexpr int PER_ROW = L == KC ? 8 : BX * E::SIZE / 16;  // pieces in an LDS row
 
+  // Piece q = tid + i * NT of an operand lies i * STEP stored rows below piece tid and in the same place of
+  // its row, since the permutations look at row bits below STEP only.
+  static constexpr int STEP = NT / PER_ROW;
+  static_assert(S != Direct || NP == 1 || STEP % 16 == 0, "one offset serves all of a lane's pieces");
+
   const char* base;
   int64_t ld;
   int valid;
   const uint8_t* exponents;
   int64_t ld_exp;
   int tid;
-  unsigned offset[S == Direct ? NP : 1];
-  i32x4 held[S == Direct ? 1 : NP];
+  unsigned offset, offset_now;  // Direct: of the lane's first piece; in the slab being sent
+  int first_piece;
+  i32x4 resource;
+  struct Two { unsigned w[2]; };
+  std::conditional_t<S == Codes, Two, i32x4> held[S == Direct ? 1 : NP];
   int held_exp[S == Codes ? NP : 1];
 
   // stored row and piece of LDS piece q
@@ -263,75 +280,73 @@ struct Loader {
     ld_exp = o.ld_exp;
     tid = tid_;
     if constexpr (S == Direct) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        int row, piece;
-        place(tid + i * NT, row, piece);
-        // (rows behind the tile's last one are fetched as its last one again: they only reach
-        // output rows that are not stored; columns behind it as zeros)
-        if (L == KC) offset[i] = (unsigned)(min(row, valid - 1) * (int)ld + piece * 16);
-        else offset[i] = piece * 16 / E::SIZE < valid ? (unsigned)(row * (int)ld + piece * 16) : kOutside;
-      }
+      int row;
+      place(tid, row, first_piece);
+      offset = (unsigned)(row * (int)ld + first_piece * 16);
+      if (L == XC && first_piece * 16 >= valid * E::SIZE) offset = kOutside;
     }
   }
 
-  // Starts fetching slab kt; k_left = values of k from this slab on.
-  __device__ __forceinline__ void fetch(int kt, int k_left, unsigned lds) {
-    const char* at = L == KC ? base + (int64_t)kt * 128 : base + (int64_t)kt * 64 * ld;
-    if constexpr (S == Direct) {
-      const i32x4 resource = buffer_of(at);
-      const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __device__ __forceinline__ const char* slab(int kt) const {
+    return L == KC ? base + (int64_t)kt * 128 : base + (int64_t)kt * 64 * ld;
+  }
+
+  // Direct: slab kt is sent piece by piece.  k_left = values of k from this slab on.  The buffer ends with
+  // the last row's last value, so that rows behind it come as zeros; in a last slab that is cut short,
+  // so do the pieces of a KC operand behind the cut.
+  __device__ __forceinline__ void aim(int kt, int k_left) {
+    const int bytes = L == KC ? (valid - 1) * (int)ld + k_left * E::SIZE : (min(k_left, 64) - 1) * (int)ld + valid * E::SIZE;
+    resource = buffer_of(slab(kt), k_left > 0 ? bytes : 0);  // (behind the last slab: nothing but zeros)
+    offset_now = L == KC && first_piece * 16 >= k_left * E::SIZE ? kOutside : offset;
+  }
+  __device__ __forceinline__ void send(int i, unsigned lds) {
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (PIECES % NT != 0 && (wave + i * (NT / 64)) * 64 >= PIECES) return;
+    load_to_lds(resource, offset_now, (unsigned)(i * STEP * (int)ld), lds + wave * 1024 + i * NT * 16);
+  }
+
+  // Staged and Codes: slab kt comes to registers.
+  __device__ __forceinline__ void fetch(int kt, int k_left) {
+    const char* at = slab(kt);
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (PIECES % NT != 0 && (wave + i * (NT / 64)) * 64 >= PIECES) break;
-        int row, piece;
-        place(tid + i * NT, row, piece);
-        const bool inside = L == KC ? piece * 16 < k_left * E::SIZE : row < k_left;
-        load_to_lds(resource, inside ? offset[i] : kOutside, lds + (wave * 64 + i * NT) * 16);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int q = tid + i * NT;
-        if (PIECES % NT != 0 && q >= PIECES) break;
-        int row, piece;
-        place(q, row, piece);
-        if constexpr (S == Staged) {
-          if (L == KC) {
-            const int r = min(row, valid - 1);
-            held[i] = load_bytes(at + r * ld + piece * 16, k_left * E::SIZE - piece * 16);
-          } else {
-            held[i] = row < k_left ? load_bytes(at + row * ld + piece * 16, valid * E::SIZE - piece * 16) : i32x4{0, 0, 0, 0};
-          }
+    for (int i = 0; i < NP; ++i) {
+      const int q = tid + i * NT;
+      if (PIECES % NT != 0 && q >= PIECES) break;
+      int row, piece;
+      place(q, row, piece);
+      if constexpr (S == Staged) {
+        if (L == KC) {
+          const int r = min(row, valid - 1);  // rows behind the last one only reach results that are not stored
+          held[i] = load_bytes(at + r * ld + piece * 16, k_left * E::SIZE - piece * 16);
         } else {
-          // eight codes for a piece of eight 16-bit values
-          const int count = row < k_left ? valid - piece * 8 : 0;
-          held[i] = i32x4{0, 0, 0, 0};
-          held_exp[i] = 0;
-          if (count > 0) {
-            const char* p = at + row * ld + piece * 8;
-            held_exp[i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (piece >> 4)];
-            if (count >= 8) {
-              __builtin_memcpy(&held[i], p, 8);
-            } else {
-              char b[8];
+          held[i] = row < k_left ? load_bytes(at + row * ld + piece * 16, valid * E::SIZE - piece * 16) : i32x4{0, 0, 0, 0};
+        }
+      } else if constexpr (S == Codes) {
+        // eight codes for a piece of eight 16-bit values
+        const int count = row < k_left ? valid - piece * 8 : 0;
+        held[i] = Two{};
+        held_exp[i] = 0;
+        if (count > 0) {
+          const char* p = at + row * ld + piece * 8;
+          held_exp[i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (piece >> 4)];
+          if (count >= 8) {
+            __builtin_memcpy(&held[i], p, 8);
+          } else {
+            char b[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
-              __builtin_memcpy(&held[i], b, 8);
-            }
+            for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
+            __builtin_memcpy(&held[i], b, 8);
           }
         }
       }
     }
   }
 
-  // Staged and Codes: what fetch() brought goes to LDS.
-  __device__ __forceinline__ void put(char* lds) {
+  // ... and piece i of it goes on to LDS.
+  __device__ __forceinline__ void put(int i, char* lds) {
+    const int q = tid + i * NT;
     if constexpr (S != Direct) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int q = tid + i * NT;
-        if (PIECES % NT != 0 && q >= PIECES) break;
+      if (PIECES % NT == 0 || q < PIECES) {
         if constexpr (S == Staged) {
           *reinterpret_cast<i32x4*>(lds + q * 16) = held[i];
         } else {
@@ -341,7 +356,7 @@ struct Loader {
           typename E::Scalar v[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            v[j] = (typename E::Scalar)((float)(int8_t)((unsigned)held[i][j >> 2] >> (8 * (j & 3))) * step);
+            v[j] = (typename E::Scalar)((float)(int8_t)(held[i].w[j >> 2] >> (8 * (j & 3))) * step);
           __builtin_memcpy(lds + q * 16, v, 16);
         }
       }
@@ -384,6 +399,11 @@ struct ProductTile {
 };
 
 // acc = sum over k of R[r, k] C[c, k] of one tile.
+//
+// A slab is two steps of the matrix instruction's k.  While a wavefront multiplies one step's fragments,
+// the next step's come from LDS into other registers, and two slabs are in LDS or on their way.  What
+// moves data is dealt out between the rows of matrix instructions: a wavefront issues in order, and the
+// loads of a whole slab in a row would keep it from issuing anything else for as long as they take.
 template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg>
 struct TileProduct {
   using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false>;
@@ -392,16 +412,30 @@ struct TileProduct {
   static_assert(LoadR::SLAB_K == LoadC::SLAB_K, "one slab for both operands");
   static constexpr int STAGE = LoadR::BYTES + LoadC::BYTES;
   static constexpr int LDS_BYTES = 2 * STAGE;
+  static constexpr int TR = Cfg::TR, TC = Cfg::TC, READS = TR + TC;
+  static constexpr int PIECES = LoadR::NP + LoadC::NP;  // that a lane moves per slab
   using Acc = typename E::Acc;
 
-  static __device__ __forceinline__ void run(const Operand& r, const Operand& c, int k_count, char* lds,
-                                             Acc (&acc)[Cfg::TR][Cfg::TC]) {
+  struct Fragments {
+    i32x4 r[TR], c[TC];
+  };
+  // Fragment number n of a step: the columns' first, then the rows'.
+  static __device__ __forceinline__ void read(Fragments& f, int n, const char* stage, int wr0, int wc0, int ks, int lane) {
+    if (n < TC) f.c[n] = LoadC::fragment(stage + LoadR::BYTES, wc0, n, ks, lane);
+    else f.r[n - TC] = LoadR::fragment(stage, wr0, n - TC, ks, lane);
+  }
+  static __device__ __forceinline__ void multiply_row(const Fragments& f, int j, Acc (&acc)[TR][TC]) {
+#pragma unroll
+    for (int i = 0; i < TC; ++i) acc[j][i] = E::mma(f.c[i], f.r[j], acc[j][i]);
+  }
+
+  static __device__ __forceinline__ void run(const Operand& r, const Operand& c, int k_count, char* lds, Acc (&acc)[TR][TC]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wr0 = (wave % Cfg::WR) * (Cfg::TR * 16), wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
+    const int wr0 = (wave % Cfg::WR) * (TR * 16), wc0 = (wave / Cfg::WR) * (TC * 16);
 #pragma unroll
-    for (int j = 0; j < Cfg::TR; ++j)
+    for (int j = 0; j < TR; ++j)
 #pragma unroll
-      for (int i = 0; i < Cfg::TC; ++i) acc[j][i] = Acc{0, 0, 0, 0};
+      for (int i = 0; i < TC; ++i) acc[j][i] = Acc{0, 0, 0, 0};
     const int slabs = (k_count + SLAB_K - 1) / SLAB_K;
     if (slabs == 0) return;
     const unsigned lds_address = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -409,40 +443,73 @@ struct TileProduct {
     LoadC lc;
     lr.init(r, tid);
     lc.init(c, tid);
-    lr.fetch(0, k_count, lds_address);
-    lc.fetch(0, k_count, lds_address + LoadR::BYTES);
-    lr.put(lds);
-    lc.put(lds + LoadR::BYTES);
-    wait_direct();
-    __syncthreads();
-    for (int kt = 0; kt < slabs; ++kt) {
-      const int here = (kt & 1) * STAGE, next = STAGE - here;
-      const bool more = kt + 1 < slabs;
-      if (more) {
-        lr.fetch(kt + 1, k_count - (kt + 1) * SLAB_K, lds_address + next);
-        lc.fetch(kt + 1, k_count - (kt + 1) * SLAB_K, lds_address + next + LoadR::BYTES);
+    auto aim = [&](int kt) {
+      if constexpr (SR == Direct) lr.aim(kt, k_count - kt * SLAB_K);
+      if constexpr (SC == Direct) lc.aim(kt, k_count - kt * SLAB_K);
+    };
+    auto fetch = [&](int kt) {
+      if constexpr (SR != Direct) lr.fetch(kt, k_count - kt * SLAB_K);
+      if constexpr (SC != Direct) lc.fetch(kt, k_count - kt * SLAB_K);
+    };
+    // piece n of slab kt on its last way: sent from memory, or put from registers
+    auto move = [&](int n, int kt) {
+      const int stage = (kt & 1) * STAGE;
+      if (n < LoadR::NP) {
+        if constexpr (SR == Direct) lr.send(n, lds_address + stage);
+        else lr.put(n, lds + stage);
+      } else {
+        if constexpr (SC == Direct) lc.send(n - LoadR::NP, lds_address + stage + LoadR::BYTES);
+        else lc.put(n - LoadR::NP, lds + stage + LoadR::BYTES);
       }
-      const char* sr = lds + here;
-      const char* sc = sr + LoadR::BYTES;
+    };
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x4 fr[Cfg::TR], fc[Cfg::TC];
+    for (int kt = 0; kt < 2; ++kt)
+      if (kt < slabs) {
+        aim(kt);
+        fetch(kt);
 #pragma unroll
-        for (int i = 0; i < Cfg::TC; ++i) fc[i] = LoadC::fragment(sc, wc0, i, ks, lane);
-#pragma unroll
-        for (int j = 0; j < Cfg::TR; ++j) fr[j] = LoadR::fragment(sr, wr0, j, ks, lane);
-#pragma unroll
-        for (int j = 0; j < Cfg::TR; ++j)
-#pragma unroll
-          for (int i = 0; i < Cfg::TC; ++i) acc[j][i] = E::mma(fc[i], fr[j], acc[j][i]);
+        for (int n = 0; n < PIECES; ++n) move(n, kt);
       }
-      if (more) {
-        lr.put(lds + next);
-        lc.put(lds + next + LoadR::BYTES);
+    fetch(2);
+    wait_arrived();
+    Fragments f0, f1;
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(f0, n, lds, wr0, wc0, 0, lane);
+    for (int kt = 0; kt + 1 < slabs; ++kt) {
+      const char* stage = lds + (kt & 1) * STAGE;
+      const char* next = lds + ((kt + 1) & 1) * STAGE;
+      // first step; the second one's fragments
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+#pragma unroll
+        for (int n = j * READS / TR; n < (j + 1) * READS / TR; ++n) read(f1, n, stage, wr0, wc0, 1, lane);
+        multiply_row(f0, j, acc);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      wait_direct();
-      __syncthreads();
+      // Every wavefront has read slab kt, and slab kt + 1 has arrived.
+      wait_arrived();
+      aim(kt + 2);
+      // second step; the next slab's first fragments, and the slab after that into the place of this one
+      // (behind the last slab zeros, rather than a branch around every move)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+#pragma unroll
+        for (int n = j * READS / TR; n < (j + 1) * READS / TR; ++n) read(f0, n, next, wr0, wc0, 0, lane);
+#pragma unroll
+        for (int n = j * PIECES / TR; n < (j + 1) * PIECES / TR; ++n) move(n, kt + 2);
+        multiply_row(f1, j, acc);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fetch(kt + 3);
     }
+    const char* last = lds + ((slabs - 1) & 1) * STAGE;
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(f1, n, last, wr0, wc0, 1, lane);
+#pragma unroll
+    for (int j = 0; j < TR; ++j) multiply_row(f0, j, acc);
+#pragma unroll
+    for (int j = 0; j < TR; ++j) multiply_row(f1, j, acc);
+    wait_loads<0>();  // no load may write to LDS once the workgroup has given it back
   }
 };
 

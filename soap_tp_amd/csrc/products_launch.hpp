@@ -37,7 +37,8 @@ template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
   const int64_t each = p.groups.tokens / std::max(1, p.groups.experts);  // rows of an average expert
   const int64_t wide_tiles = ceil_div64(p.groups.tokens, 256) * ceil_div64(p.cols, 256);
-  if (each >= 192 && wide_tiles >= 192) return launch_rows<E, LC, S, WideTile>(stream, p);
+  if constexpr (S == Direct)
+    if (each >= 192 && wide_tiles >= 192) return launch_rows<E, LC, S, WideTile>(stream, p);
   if (each > 48) return launch_rows<E, LC, S, MidTile>(stream, p);
   return launch_rows<E, LC, S, LowTile>(stream, p);
 }
@@ -63,7 +64,8 @@ int launch_sums(hipStream_t stream, SumProblem p) {
 template <class E, Source SR, Source SC>
 int launch_sums(hipStream_t stream, const SumProblem& p) {
   const int64_t wide_tiles = ceil_div64(p.rows, 256) * ceil_div64(p.cols, 256) * p.groups.experts;
-  if (wide_tiles >= 192) return launch_sums<E, SR, SC, WideTile>(stream, p);
+  if constexpr (SR == Direct)
+    if (wide_tiles >= 192) return launch_sums<E, SR, SC, WideTile>(stream, p);
   return launch_sums<E, SR, SC, MidTile>(stream, p);
 }
 
