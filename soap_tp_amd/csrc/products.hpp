@@ -95,11 +95,13 @@ struct RowTile {
   int rows;    // rows of the tile that belong to the group (1 .. BR)
 };
 
-// Tile number wg of the launch -> its rows and columns.  Row tiles never cross a group's end.
+// Tile number wg of the launch -> its rows and columns.  Row tiles never cross a group's end; a group of
+// n rows has ceil(n / BR) of them, which share its rows evenly in units of GRAIN: a tile's time goes by
+// its rows (see TileProduct), and one nearly empty tile behind full ones would be a round of its own.
 // Consecutive workgroup ids are dealt round-robin to the 8 XCDs; each XCD gets one contiguous range of
 // tiles, walked in groups of up to 8 row tiles by all columns, so that a weight tile is fetched into
 // that XCD's L2 once for its row tiles.  Returns false behind the last tile.
-template <int BR>
+template <int BR, int GRAIN>
 __device__ __forceinline__ bool locate_rows(const RowGroups& g, int tiles_c, int wg, RowTile& tile, int& tile_c) {
   const int lane = threadIdx.x & 63;
   const int groups = g.experts + g.rest;
@@ -141,9 +143,13 @@ __device__ __forceinline__ bool locate_rows(const RowGroups& g, int tiles_c, int
       const int up_to = at ? __shfl(tiles, at - 1) : 0;
       begin = __shfl(begin, at);
       end = __shfl(end, at);
+      const int count = end - begin, share = (count + BR - 1) / BR, nth = tr - before - up_to;
+      const int64_t grains = (count + GRAIN - 1) / GRAIN;
+      const int first = (int)(nth * grains / share) * GRAIN;
+      const int last = min(count, (int)((nth + 1) * grains / share) * GRAIN);
       tile.expert = __builtin_amdgcn_readfirstlane(e0 + at);
-      tile.row = __builtin_amdgcn_readfirstlane(begin + (tr - before - up_to) * BR);
-      tile.rows = __builtin_amdgcn_readfirstlane(min(BR, end - (begin + (tr - before - up_to) * BR)));
+      tile.row = __builtin_amdgcn_readfirstlane(begin + first);
+      tile.rows = __builtin_amdgcn_readfirstlane(last - first);
       return true;
     }
     before += __shfl(tiles, 63);
@@ -305,11 +311,12 @@ struct Loader {
     load_to_lds(resource, offset_now, (unsigned)(i * STEP * (int)ld), lds + wave * 1024 + i * NT * 16);
   }
 
-  // Staged and Codes: slab kt comes to registers.
+  // Staged and Codes: a lane's first COUNT pieces of slab kt come to registers.
+  template <int COUNT>
   __device__ __forceinline__ void fetch(int kt, int k_left) {
     const char* at = slab(kt);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
+    for (int i = 0; i < COUNT; ++i) {
       const int q = tid + i * NT;
       if (PIECES % NT != 0 && q >= PIECES) break;
       int row, piece;
@@ -398,13 +405,15 @@ struct ProductTile {
   static_assert(BR % (16 * WR) == 0 && BC % (16 * WC) == 0, "wave tiling");
 };
 
-// acc = sum over k of R[r, k] C[c, k] of one tile.
+// acc = sum over k of R[r, k] C[c, k] of one tile, of which the first A * WR fragments of 16 rows are
+// computed.  The fragments are dealt to the WR rows of wavefronts in turn, so that a tile with few rows
+// takes all of them for a shorter time.
 //
 // A slab is two steps of the matrix instruction's k.  While a wavefront multiplies one step's fragments,
 // the next step's come from LDS into other registers, and two slabs are in LDS or on their way.  What
 // moves data is dealt out between the rows of matrix instructions: a wavefront issues in order, and the
 // loads of a whole slab in a row would keep it from issuing anything else for as long as they take.
-template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg>
+template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg, int A = Cfg::TR>
 struct TileProduct {
   using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false>;
   using LoadC = Loader<E, LC, SC, Cfg::BC, Cfg::NT, true>;
@@ -412,8 +421,10 @@ struct TileProduct {
   static_assert(LoadR::SLAB_K == LoadC::SLAB_K, "one slab for both operands");
   static constexpr int STAGE = LoadR::BYTES + LoadC::BYTES;
   static constexpr int LDS_BYTES = 2 * STAGE;
-  static constexpr int TR = Cfg::TR, TC = Cfg::TC, READS = TR + TC;
-  static constexpr int PIECES = LoadR::NP + LoadC::NP;  // that a lane moves per slab
+  static constexpr int TR = A, TC = Cfg::TC, READS = TR + TC;
+  // pieces that a lane moves per slab: of a KC row operand only those of the rows that are computed
+  static constexpr int PIECES_R = LR == KC ? (A * Cfg::WR * 16 + LoadR::STEP - 1) / LoadR::STEP : LoadR::NP;
+  static constexpr int PIECES = PIECES_R + LoadC::NP;
   using Acc = typename E::Acc;
 
   struct Fragments {
@@ -422,7 +433,7 @@ struct TileProduct {
   // Fragment number n of a step: the columns' first, then the rows'.
   static __device__ __forceinline__ void read(Fragments& f, int n, const char* stage, int wr0, int wc0, int ks, int lane) {
     if (n < TC) f.c[n] = LoadC::fragment(stage + LoadR::BYTES, wc0, n, ks, lane);
-    else f.r[n - TC] = LoadR::fragment(stage, wr0, n - TC, ks, lane);
+    else f.r[n - TC] = LoadR::fragment(stage, wr0, (n - TC) * Cfg::WR, ks, lane);
   }
   static __device__ __forceinline__ void multiply_row(const Fragments& f, int j, Acc (&acc)[TR][TC]) {
 #pragma unroll
@@ -431,7 +442,7 @@ struct TileProduct {
 
   static __device__ __forceinline__ void run(const Operand& r, const Operand& c, int k_count, char* lds, Acc (&acc)[TR][TC]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wr0 = (wave % Cfg::WR) * (TR * 16), wc0 = (wave / Cfg::WR) * (TC * 16);
+    const int wr0 = (wave % Cfg::WR) * 16, wc0 = (wave / Cfg::WR) * (TC * 16);
 #pragma unroll
     for (int j = 0; j < TR; ++j)
 #pragma unroll
@@ -448,18 +459,18 @@ struct TileProduct {
       if constexpr (SC == Direct) lc.aim(kt, k_count - kt * SLAB_K);
     };
     auto fetch = [&](int kt) {
-      if constexpr (SR != Direct) lr.fetch(kt, k_count - kt * SLAB_K);
-      if constexpr (SC != Direct) lc.fetch(kt, k_count - kt * SLAB_K);
+      if constexpr (SR != Direct) lr.template fetch<PIECES_R>(kt, k_count - kt * SLAB_K);
+      if constexpr (SC != Direct) lc.template fetch<LoadC::NP>(kt, k_count - kt * SLAB_K);
     };
     // piece n of slab kt on its last way: sent from memory, or put from registers
     auto move = [&](int n, int kt) {
       const int stage = (kt & 1) * STAGE;
-      if (n < LoadR::NP) {
+      if (n < PIECES_R) {
         if constexpr (SR == Direct) lr.send(n, lds_address + stage);
         else lr.put(n, lds + stage);
       } else {
-        if constexpr (SC == Direct) lc.send(n - LoadR::NP, lds_address + stage + LoadR::BYTES);
-        else lc.put(n - LoadR::NP, lds + stage + LoadR::BYTES);
+        if constexpr (SC == Direct) lc.send(n - PIECES_R, lds_address + stage + LoadR::BYTES);
+        else lc.put(n - PIECES_R, lds + stage + LoadR::BYTES);
       }
     };
 #pragma unroll
@@ -542,14 +553,14 @@ __device__ __forceinline__ void store_eight(void* base, int64_t at, const float 
 }
 
 // scale: (row of tile, column of tile, accumulator) -> result.
-template <class Cfg, class Acc, class Scale>
-__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[Cfg::TR][Cfg::TC], const Scale& scale) {
+template <class Cfg, int A, class Acc, class Scale>
+__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[A][Cfg::TC], const Scale& scale) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = lane & 15, g = lane >> 4;
-  const int wr0 = (wave % Cfg::WR) * (Cfg::TR * 16), wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
+  const int wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
 #pragma unroll
-  for (int j = 0; j < Cfg::TR; ++j) {
-    const int r = wr0 + 16 * j + m;
+  for (int j = 0; j < A; ++j) {
+    const int r = (Cfg::WR * j + wave % Cfg::WR) * 16 + m;
     if (r >= o.rows) continue;
 #pragma unroll
     for (int i = 0; i < Cfg::TC; i += 2) {
@@ -602,15 +613,9 @@ struct RowProblem {
 
 __device__ __forceinline__ int type_bytes(int type) { return type == kFloat32 ? 4 : 2; }
 
-template <class E, Layout LC, Source S, class Cfg>
-__global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
-  using Product = TileProduct<E, KC, S, LC, S, Cfg>;
-  __shared__ __attribute__((aligned(1024))) char lds[Product::LDS_BYTES];
-  RowTile tile;
-  int tile_c;
-  if (!locate_rows<Cfg::BR>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
-  const int c0 = tile_c * Cfg::BC;
-  const bool rest = tile.expert >= p.groups.experts;
+// The tile with A fragments of rows for each row of wavefronts.
+template <class E, Layout LC, Source S, class Cfg, int A>
+__device__ __forceinline__ void row_tile(const RowProblem& p, const RowTile& tile, int c0, char* lds) {
   Operand r, c;
   r.base = p.r + (int64_t)tile.row * p.ldr;
   r.ld = p.ldr;
@@ -620,8 +625,8 @@ __global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
   c.valid = min(Cfg::BC, p.cols - c0);
   r.exponents = c.exponents = nullptr;
   r.ld_exp = c.ld_exp = 0;
-  typename E::Acc acc[Cfg::TR][Cfg::TC];
-  Product::run(r, c, rest ? 0 : p.k, lds, acc);
+  typename E::Acc acc[A][Cfg::TC];
+  TileProduct<E, KC, S, LC, S, Cfg, A>::run(r, c, tile.expert >= p.groups.experts ? 0 : p.k, lds, acc);
   Result o;
   o.base = static_cast<char*>(p.y) + ((int64_t)tile.row * p.ldy + c0) * type_bytes(p.out_type);
   o.ld = p.ldy;
@@ -630,9 +635,133 @@ __global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
   o.type = p.out_type;
   o.wide = p.wide;
   if constexpr (E::SIZE == 1)
-    store_tile<Cfg>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0});
+    store_tile<Cfg, A>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0});
   else
-    store_tile<Cfg>(o, acc, Unscaled{});
+    store_tile<Cfg, A>(o, acc, Unscaled{});
+}
+
+template <class E, Layout LC, Source S, class Cfg, int A>
+__device__ __forceinline__ void row_tile_at_least(const RowProblem& p, const RowTile& tile, int c0, int fragments, char* lds) {
+  constexpr int LESS = A > 4 ? A - 1 : A - 2;  // 8, 7, 6, 5, 4, 2
+  if constexpr (LESS >= 1)
+    if (fragments <= LESS) return row_tile_at_least<E, LC, S, Cfg, LESS>(p, tile, c0, fragments, lds);
+  row_tile<E, LC, S, Cfg, A>(p, tile, c0, lds);
+}
+
+template <class E, Layout LC, Source S, class Cfg>
+__global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
+  __shared__ __attribute__((aligned(1024))) char lds[TileProduct<E, KC, S, LC, S, Cfg>::LDS_BYTES];
+  constexpr int GRAIN = 16 * Cfg::WR;
+  RowTile tile;
+  int tile_c;
+  if (!locate_rows<Cfg::BR, GRAIN>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
+  row_tile_at_least<E, LC, S, Cfg, Cfg::TR>(p, tile, tile_c * Cfg::BC, (tile.rows + GRAIN - 1) / GRAIN, lds);
+}
+
+// ---- few rows ------------------------------------------------------------------------------
+//
+// With a handful of rows for an expert the product is the reading of its weights (k contiguous).  A
+// workgroup has 32 outputs and up to 32 rows of one expert; its eight wavefronts take every eighth 128
+// bytes of k, straight from memory to the matrix instruction's registers: no wavefront waits for
+// another one before the end, so all of a compute unit's loads are in flight at once.  The eight sums
+// meet in LDS and are added in order.
+struct FewTile {
+  static constexpr int BR = 32, BC = 32, WAVES = 8, NT = 64 * WAVES;
+  static constexpr int BATCH = 4;  // steps of 128 bytes that a wavefront has in flight
+};
+
+template <class E, int A>
+__device__ __forceinline__ void few_rows_tile(const RowProblem& p, const RowTile& tile, int c0, int k, char* lds) {
+  using Acc = typename E::Acc;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m = lane & 15, g = lane >> 4;
+  const int64_t bytes = (int64_t)k * E::SIZE;
+  const int cols = min(FewTile::BC, p.cols - c0);
+  // (rows and columns behind the last one are read as the last one again and not stored)
+  const char* w[2];
+  const char* x[A];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = p.c + (int64_t)tile.expert * p.stride_c + (int64_t)(c0 + min(16 * i + m, cols - 1)) * p.ldc + g * 16;
+#pragma unroll
+  for (int j = 0; j < A; ++j) x[j] = p.r + (int64_t)(tile.row + min(16 * j + m, tile.rows - 1)) * p.ldr + g * 16;
+  Acc acc[A][2];
+#pragma unroll
+  for (int j = 0; j < A; ++j) acc[j][0] = acc[j][1] = Acc{0, 0, 0, 0};
+  const int steps = (int)(bytes >> 7);  // whole ones
+  int s = wave;
+  for (; s + (FewTile::BATCH - 1) * FewTile::WAVES < steps; s += FewTile::BATCH * FewTile::WAVES) {
+    i32x4 fw[FewTile::BATCH][2][2], fx[FewTile::BATCH][A][2];
+#pragma unroll
+    for (int b = 0; b < FewTile::BATCH; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t at = (int64_t)(s + b * FewTile::WAVES) * 128 + h * 64;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) __builtin_memcpy(&fw[b][i][h], w[i] + at, 16);
+#pragma unroll
+        for (int j = 0; j < A; ++j) __builtin_memcpy(&fx[b][j][h], x[j] + at, 16);
+      }
+#pragma unroll
+    for (int b = 0; b < FewTile::BATCH; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < A; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[j][i] = E::mma(fw[b][i][h], fx[b][j][h], acc[j][i]);
+  }
+  for (; s * (int64_t)128 < bytes; s += FewTile::WAVES) {  // the remaining steps, the last of them perhaps cut short
+    i32x4 fw[2][2], fx[A][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t at = (int64_t)s * 128 + h * 64;
+      const int count = (int)min((int64_t)16, bytes - at - g * 16);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fw[i][h] = load_bytes(w[i] + at, count);
+#pragma unroll
+      for (int j = 0; j < A; ++j) fx[j][h] = load_bytes(x[j] + at, count);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < A; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[j][i] = E::mma(fw[i][h], fx[j][h], acc[j][i]);
+  }
+  // sums[wave][row][output], outputs padded so that a fragment's four rows of lanes fall on different banks
+  using Sum = std::conditional_t<E::SIZE == 1, int, float>;
+  constexpr int STRIDE = FewTile::BC + 4;
+  Sum* sums = reinterpret_cast<Sum*>(lds);
+#pragma unroll
+  for (int j = 0; j < A; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<Acc*>(sums + ((wave * A + j) * 16 + m) * STRIDE + 16 * i + 4 * g) = acc[j][i];
+  __syncthreads();
+#pragma unroll
+  for (int at = tid; at < A * 16 * FewTile::BC; at += FewTile::NT) {
+    const int r = at / FewTile::BC, c = at % FewTile::BC;
+    if (r >= tile.rows || c >= cols) continue;
+    Sum v = 0;
+#pragma unroll
+    for (int q = 0; q < FewTile::WAVES; ++q) v += sums[(q * A * 16 + r) * STRIDE + c];
+    float out;
+    if constexpr (E::SIZE == 1) out = TokenChannel{p.token_scale + tile.row, p.channel_scale + c0}(r, c, v);
+    else out = v;
+    store_value(p.y, (int64_t)(tile.row + r) * p.ldy + c0 + c, p.out_type, out);
+  }
+}
+
+template <class E>
+__global__ __launch_bounds__(FewTile::NT) void few_rows_kernel(RowProblem p) {
+  __shared__ __attribute__((aligned(16))) char lds[FewTile::WAVES * FewTile::BR * (FewTile::BC + 4) * 4];
+  RowTile tile;
+  int tile_c;
+  if (!locate_rows<FewTile::BR, 16>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
+  const int k = tile.expert >= p.groups.experts ? 0 : p.k, c0 = tile_c * FewTile::BC;
+  if (tile.rows <= 16) few_rows_tile<E, 1>(p, tile, c0, k, lds);
+  else few_rows_tile<E, 2>(p, tile, c0, k, lds);
 }
 
 struct SumProblem {
@@ -699,7 +828,7 @@ __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
   o.cols = c.valid;
   o.type = p.out_type;
   o.wide = p.wide;
-  store_tile<Cfg>(o, acc, Unscaled{});
+  store_tile<Cfg, Cfg::TR>(o, acc, Unscaled{});
 }
 
 // ---- fp32 ----------------------------------------------------------------------------------
@@ -727,7 +856,7 @@ __global__ __launch_bounds__(Cfg::NT) void row_product_f32_kernel(RowProblem p, 
   __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
   RowTile tile;
   int tile_c;
-  if (!locate_rows<Cfg::BN>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
+  if (!locate_rows<Cfg::BN, Cfg::BN>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
   const int c0 = tile_c * Cfg::BM;
   const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
   const float* w = reinterpret_cast<const float*>(p.c + (int64_t)tile.expert * p.stride_c) +

@@ -33,6 +33,16 @@ int launch_rows(hipStream_t stream, RowProblem p) {
   return kOk;
 }
 
+template <class E>
+int launch_few_rows(hipStream_t stream, RowProblem p) {
+  p.tiles_c = (int)ceil_div64(p.cols, FewTile::BC);
+  unsigned grid;
+  if (int rc = grid_of(most_row_tiles(p.groups, FewTile::BR) * p.tiles_c, &grid)) return rc;
+  hipLaunchKernelGGL((few_rows_kernel<E>), dim3(grid), dim3(FewTile::NT), 0, stream, p);
+  SOAPMI_LAUNCH_CHECK();
+  return kOk;
+}
+
 template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
   const int64_t each = p.groups.tokens / std::max(1, p.groups.experts);  // rows of an average expert
@@ -46,6 +56,8 @@ int launch_rows(hipStream_t stream, const RowProblem& p) {
 // Y = rows times their expert's matrices.  direct: both operands may be fetched straight to LDS.
 template <class E, Layout LC>
 int row_products(hipStream_t stream, const RowProblem& p, bool direct) {
+  if constexpr (LC == KC)
+    if (p.groups.tokens <= (int64_t)32 * std::max(1, p.groups.experts)) return launch_few_rows<E>(stream, p);
   return direct ? launch_rows<E, LC, Direct>(stream, p) : launch_rows<E, LC, Staged>(stream, p);
 }
 
