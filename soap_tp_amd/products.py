@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from .ops._common import native_call, require_device_tensor, stream_of
+from .ops._common import native_call, require_device_tensor
 
 __all__ = [
     "ActivationCheckpoint",
@@ -58,6 +58,27 @@ class ActivationCheckpoint(NamedTuple):
 
 
 # ---- checks --------------------------------------------------------------------------------
+#
+# A small product takes the device less time than a line-by-line description of its arguments takes the
+# host, so the checks that pass read each property once and messages are made only where one fails.
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch(index: int, name: str, *arguments) -> None:
+    """Call an entry point on torch's current stream of device ``index``."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(index, name, *arguments)
+    native_call(name, *arguments, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index))
+
+
+def _refuse_devices(device: torch.device, **tensors: Optional[Tensor]) -> None:
+    for name, tensor in tensors.items():
+        if tensor is not None:
+            if tensor.device != device:
+                raise ValueError(f"{name} is on {tensor.device}, expected {device}.")
+            require_device_tensor(name, tensor)
 
 
 def _check_matrix(name: str, tensor: Tensor, dimensions: int = 2) -> None:
@@ -67,38 +88,31 @@ def _check_matrix(name: str, tensor: Tensor, dimensions: int = 2) -> None:
         raise ValueError(f"{name} must be {dimensions}D, got {tensor.ndim}D.")
 
 
-def _check_values(name: str, tensor: Tensor, dimensions: int = 2) -> None:
+def _check_values(name: str, tensor: Tensor, dimensions: int = 2) -> int:
+    """The code of the tensor's type."""
     _check_matrix(name, tensor, dimensions)
-    if tensor.dtype not in _DTYPES:
+    code = _DTYPES.get(tensor.dtype)
+    if code is None:
         raise ValueError(f"{name} must use float32, bfloat16 or float16, got {tensor.dtype}.")
-
-
-def _check_together(device: torch.device, **tensors: Tensor) -> None:
-    for name, tensor in tensors.items():
-        if tensor.device != device:
-            raise ValueError(f"{name} is on {tensor.device}, expected {device}.")
-        require_device_tensor(name, tensor)
+    return code
 
 
 def _rows(tensor: Tensor) -> Tuple[Tensor, int]:
     """The tensor with its last dimension contiguous (copied if it is not) and its row stride."""
-    columns = tensor.size(-1)
-    stride = tensor.stride(-2) if tensor.size(-2) > 1 else max(1, columns)
-    if (columns > 1 and tensor.stride(-1) != 1) or stride < max(1, columns):
-        tensor = tensor.contiguous()
-        stride = max(1, columns)
-    return tensor, stride
+    rows, columns = tensor.shape[-2:]
+    strides = tensor.stride()
+    if rows <= 1:
+        if columns <= 1 or strides[-1] == 1:
+            return tensor, max(1, columns)
+    elif strides[-2] >= max(1, columns) and (columns <= 1 or strides[-1] == 1):
+        return tensor, strides[-2]
+    return tensor.contiguous(), max(1, columns)
 
 
 def _experts(tensor: Tensor) -> Tuple[Tensor, int, int]:
     """Weights as (tensor, row stride, expert stride)."""
     tensor, row = _rows(tensor)
-    if tensor.ndim == 2:
-        return tensor, row, 0
-    if tensor.size(0) > 1 and tensor.stride(0) < 0:
-        tensor = tensor.contiguous()
-        row = max(1, tensor.size(-1))
-    return tensor, row, tensor.stride(0) if tensor.size(0) > 1 else 0
+    return tensor, row, tensor.stride(0) if tensor.ndim == 3 and tensor.size(0) > 1 else 0
 
 
 def _check_ends(ends: Optional[Tensor], experts: int) -> int:
@@ -109,7 +123,7 @@ def _check_ends(ends: Optional[Tensor], experts: int) -> int:
         raise ValueError(f"ends must use int64, got {ends.dtype}.")
     if ends.numel() != experts:
         raise ValueError(f"ends has {ends.numel()} entries, expected one for each of {experts} experts.")
-    if ends.numel() > 1 and ends.stride(0) != 1:
+    if experts > 1 and ends.stride(0) != 1:
         raise ValueError("ends must be contiguous.")
     return ends.data_ptr()
 
@@ -117,29 +131,31 @@ def _check_ends(ends: Optional[Tensor], experts: int) -> int:
 def _spans(tensor: Tensor) -> Tuple[int, int]:
     """First and last byte of memory that a tensor's elements use."""
     first = tensor.data_ptr()
-    reach = sum((size - 1) * abs(stride) for size, stride in zip(tensor.shape, tensor.stride()))
+    reach = sum((size - 1) * stride for size, stride in zip(tensor.shape, tensor.stride()))
     return first, first + (reach + 1) * tensor.element_size()
 
 
-def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, ...], **inputs: Tensor) -> None:
-    """``out`` as a caller gave it: rows of contiguous values, written in place, apart from the inputs."""
+def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, ...], **inputs: Optional[Tensor]) -> int:
+    """``out`` as a caller gave it: rows of contiguous values, written in place, apart from the inputs.
+    The code of its type."""
     _check_matrix("out", out, len(shape))
     if tuple(out.shape) != shape:
         raise ValueError(f"out has shape {tuple(out.shape)}, expected {shape}.")
     if out.dtype not in dtypes:
         raise ValueError(f"out must use {' or '.join(str(d) for d in dtypes)}, got {out.dtype}.")
-    if out.numel() == 0:
-        return
-    if (shape[-1] > 1 and out.stride(-1) != 1) or (shape[-2] > 1 and out.stride(-2) < shape[-1]):
-        raise ValueError("out must have contiguous rows that do not overlap.")
-    if len(shape) == 3 and shape[0] > 1 and out.stride(0) < (shape[1] - 1) * out.stride(1) + shape[2]:
-        raise ValueError("out must have matrices that do not overlap.")
-    first, last = _spans(out)
-    for name, tensor in inputs.items():
-        if tensor is not None and tensor.numel():
-            low, high = _spans(tensor)
-            if low < last and first < high:
-                raise ValueError(f"out must not overlap {name}.")
+    if out.numel():
+        strides = out.stride()
+        if (shape[-1] > 1 and strides[-1] != 1) or (shape[-2] > 1 and strides[-2] < shape[-1]):
+            raise ValueError("out must have contiguous rows that do not overlap.")
+        if len(shape) == 3 and shape[0] > 1 and strides[0] < (shape[1] - 1) * _row_stride(out) + shape[2]:
+            raise ValueError("out must have matrices that do not overlap.")
+        first, last = _spans(out)
+        for name, tensor in inputs.items():
+            if tensor is not None and tensor.numel():
+                low, high = _spans(tensor)
+                if low < last and first < high:
+                    raise ValueError(f"out must not overlap {name}.")
+    return _DTYPES[out.dtype]
 
 
 def _row_stride(tensor: Tensor) -> int:
@@ -153,57 +169,50 @@ def _out_types(dtype: torch.dtype) -> Tuple[torch.dtype, ...]:
 # ---- grouped products ----------------------------------------------------------------------
 
 
-def _grouped(x: Tensor, weights: Tensor, ends: Optional[Tensor], out: Optional[Tensor], transposed: bool, name: str) -> Tensor:
-    _check_values(name, x)
-    _check_values("weights", weights, 2 if ends is None else 3)
-    if weights.dtype != x.dtype:
+def _grouped(x: Tensor, weights: Tensor, ends: Optional[Tensor], out: Optional[Tensor], transposed: int, name: str) -> Tensor:
+    code = _check_values(name, x)
+    if _check_values("weights", weights, 2 if ends is None else 3) != code:
         raise ValueError(f"weights must use {x.dtype} as {name} does, got {weights.dtype}.")
+    tokens, width = x.shape
     outputs, inputs = weights.shape[-2:]
     inner, columns = (outputs, inputs) if transposed else (inputs, outputs)
-    if x.size(1) != inner:
-        raise ValueError(f"{name} has {x.size(1)} columns, expected {inner}.")
+    if width != inner:
+        raise ValueError(f"{name} has {width} columns, expected {inner}.")
     experts = 1 if ends is None else weights.size(0)
     pointer = _check_ends(ends, experts)
-    tokens = x.size(0)
-    tensors = {name: x, "weights": weights, **({} if ends is None else {"ends": ends})}
-    if out is not None:
-        _check_out(out, (tokens, columns), _out_types(x.dtype), **tensors)
-        tensors["out"] = out
-    _check_together(x.device, **tensors)
     fresh = out is None
+    out_code = code if fresh else _check_out(out, (tokens, columns), _out_types(x.dtype), **{name: x}, weights=weights, ends=ends)
+    index = x.get_device()
+    if (index < 0 or weights.get_device() != index or (pointer and ends.get_device() != index)
+            or (not fresh and out.get_device() != index)):
+        _refuse_devices(x.device, **{name: x}, weights=weights, ends=ends, out=out)
     if fresh:
         out = torch.empty((tokens, columns), dtype=x.dtype, device=x.device)
-    if out.numel() == 0:
-        return out
-    with torch.cuda.device(x.device):
+    if tokens and columns:
         rows, ldx = _rows(x)
         matrices, ldw, stride_w = _experts(weights)
-        native_call(
-            "soapmi_expert_product", _DTYPES[x.dtype], rows.data_ptr(), ldx, matrices.data_ptr(), ldw, stride_w,
-            1 if transposed else 0, pointer, experts, tokens, outputs, inputs, _DTYPES[out.dtype], out.data_ptr(),
-            _row_stride(out), 1 if fresh else 0, stream_of(x),
-        )
+        _launch(index, "soapmi_expert_product", code, rows.data_ptr(), ldx, matrices.data_ptr(), ldw, stride_w, transposed,
+                pointer, experts, tokens, outputs, inputs, out_code, out.data_ptr(), columns if fresh else _row_stride(out),
+                1 if fresh else 0)
     return out
 
 
-@torch.no_grad()
 def expert_product(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, out: Optional[Tensor] = None) -> Tensor:
     """``y[t] = W_e x[t]`` for every row ``t`` of every expert ``e``.
 
     ``x`` is (tokens, inputs), ``weights`` (experts, outputs, inputs) of the same type; the result is
     (tokens, outputs) of that type.  ``out`` receives the result instead of a new tensor and may be
-    float32.  Rows of no expert are zero in a new tensor and left as they were in ``out``."""
-    return _grouped(x, weights, ends, out, False, "x")
+    float32.  Rows of no expert are zero in a new tensor and left as they were in ``out``.  Not recorded
+    by autograd: see ``expert_linear``."""
+    return _grouped(x, weights, ends, out, 0, "x")
 
 
-@torch.no_grad()
 def expert_input_gradient(gradient: Tensor, weights: Tensor, ends: Optional[Tensor], *, out: Optional[Tensor] = None) -> Tensor:
     """``dx[t] = W_e^T dy[t]``: the gradient of ``expert_product``'s ``x`` from that of its result,
     (tokens, inputs) from (tokens, outputs); otherwise as ``expert_product``."""
-    return _grouped(gradient, weights, ends, out, True, "gradient")
+    return _grouped(gradient, weights, ends, out, 1, "gradient")
 
 
-@torch.no_grad()
 def expert_weight_gradient(
     gradient: Tensor,
     x: Union[Tensor, ActivationCheckpoint],
@@ -218,49 +227,50 @@ def expert_weight_gradient(
     ``gradient`` is (tokens, outputs); ``x`` (tokens, inputs) of the same type, or the checkpoint that
     was made from it.  The result is float32, the type ``soap_step`` takes, or ``out_dtype`` (the
     gradient's own type); ``out`` receives it instead of a new tensor."""
-    _check_values("gradient", gradient)
+    code = _check_values("gradient", gradient)
     saved = isinstance(x, ActivationCheckpoint)
     if saved:
         _check_checkpoint(x)
-        tokens, inputs, dtype = x.codes.size(0), x.codes.size(1), x.dtype
+        values, exponents, dtype = x
     else:
         _check_values("x", x)
-        tokens, inputs, dtype = x.size(0), x.size(1), x.dtype
+        values, exponents, dtype = x, None, x.dtype
     if dtype != gradient.dtype:
         raise ValueError(f"x must use {gradient.dtype} as gradient does, got {dtype}.")
-    if gradient.size(0) != tokens:
-        raise ValueError(f"gradient has {gradient.size(0)} rows, expected {tokens}.")
-    outputs = gradient.size(1)
-    if ends is not None:
+    (tokens, inputs), (rows, outputs) = values.shape, gradient.shape
+    if rows != tokens:
+        raise ValueError(f"gradient has {rows} rows, expected {tokens}.")
+    if ends is None:
+        experts, pointer, shape = 1, 0, (outputs, inputs)
+    else:
         _check_matrix("ends", ends, 1)
-    experts = 1 if ends is None else ends.numel()
-    pointer = _check_ends(ends, experts)
-    shape = (outputs, inputs) if ends is None else (experts, outputs, inputs)
-    parts = {"codes": x.codes, "exponents": x.exponents} if saved else {"x": x}
-    tensors = {"gradient": gradient, **parts, **({} if ends is None else {"ends": ends})}
+        experts = ends.numel()
+        pointer, shape = _check_ends(ends, experts), (experts, outputs, inputs)
     if out is not None:
-        _check_out(out, shape, _out_types(dtype), **tensors)
-        tensors["out"] = out
+        out_code = _check_out(out, shape, _out_types(dtype), gradient=gradient, x=values, exponents=exponents, ends=ends)
     elif out_dtype not in _out_types(dtype):
         raise ValueError(f"out_dtype must be {' or '.join(str(d) for d in _out_types(dtype))}, got {out_dtype}.")
-    _check_together(gradient.device, **tensors)
+    else:
+        out_code = _DTYPES[out_dtype]
+    index = gradient.get_device()
+    if (index < 0 or values.get_device() != index or (saved and exponents.get_device() != index)
+            or (pointer and ends.get_device() != index) or (out is not None and out.get_device() != index)):
+        _refuse_devices(gradient.device, gradient=gradient, x=values, exponents=exponents, ends=ends, out=out)
     if out is None:
         out = torch.empty(shape, dtype=out_dtype, device=gradient.device)
     if out.numel() == 0:
         return out
-    if saved and dtype == torch.float32:
-        x, saved = restore_activations(x), False  # the matrix cores take no 8-bit values beside fp32
-    stride = out.stride(0) if out.ndim == 3 and experts > 1 else 0
-    with torch.cuda.device(gradient.device):
-        rows, ldg = _rows(gradient)
-        tail = (pointer, experts, tokens, outputs, inputs, _DTYPES[out.dtype], out.data_ptr(), _row_stride(out), stride,
-                stream_of(gradient))
-        if saved:
-            native_call("soapmi_expert_weight_gradient_saved", _DTYPES[dtype], rows.data_ptr(), ldg, x.codes.data_ptr(),
-                        _row_stride(x.codes), x.exponents.data_ptr(), _row_stride(x.exponents), *tail)
-        else:
-            values, ldx = _rows(x)
-            native_call("soapmi_expert_weight_gradient", _DTYPES[dtype], rows.data_ptr(), ldg, values.data_ptr(), ldx, *tail)
+    if saved and code == 0:
+        values, saved = restore_activations(x), False  # the matrix cores take no 8-bit values beside fp32
+    gradient, ldg = _rows(gradient)
+    values, ldx = _rows(values)
+    tail = (pointer, experts, tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out),
+            out.stride(0) if experts > 1 else 0)
+    if saved:
+        _launch(index, "soapmi_expert_weight_gradient_saved", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx,
+                exponents.data_ptr(), _row_stride(exponents), *tail)
+    else:
+        _launch(index, "soapmi_expert_weight_gradient", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx, *tail)
     return out
 
 
@@ -326,66 +336,65 @@ def _check_checkpoint(checkpoint: ActivationCheckpoint) -> None:
 
 def _code_matrix(rows: int, columns: int, device) -> Tensor:
     """int8 rows that start at multiples of 16 bytes."""
+    if columns % 16 == 0:
+        return torch.empty((rows, columns), dtype=torch.int8, device=device)
     return torch.empty((rows, -(-columns // 16) * 16), dtype=torch.int8, device=device)[:, :columns]
 
 
-@torch.no_grad()
 def checkpoint_activations(x: Tensor) -> ActivationCheckpoint:
     """Keep a matrix in 8 bits, with a power-of-two step for each row and 128 columns: half the memory
     of 16-bit activations.  A value is restored to within half a step (within a step above 127.5
     steps), a step being at most 1/64 of the largest magnitude of its 128 columns."""
-    _check_values("x", x)
-    require_device_tensor("x", x)
+    code = _check_values("x", x)
+    index = x.get_device()
+    if index < 0:
+        _refuse_devices(x.device, x=x)
     rows, columns = x.shape
     codes = _code_matrix(rows, columns, x.device)
     exponents = torch.empty((rows, -(-columns // CHECKPOINT_BLOCK)), dtype=torch.uint8, device=x.device)
-    if x.numel():
-        with torch.cuda.device(x.device):
-            values, ldx = _rows(x)
-            native_call("soapmi_checkpoint_activations", _DTYPES[x.dtype], values.data_ptr(), ldx, rows, columns,
-                        codes.data_ptr(), _row_stride(codes), exponents.data_ptr(), _row_stride(exponents), stream_of(x))
+    if rows and columns:
+        values, ldx = _rows(x)
+        _launch(index, "soapmi_checkpoint_activations", code, values.data_ptr(), ldx, rows, columns, codes.data_ptr(),
+                _row_stride(codes), exponents.data_ptr(), -(-columns // CHECKPOINT_BLOCK))
     return ActivationCheckpoint(codes, exponents, x.dtype)
 
 
-@torch.no_grad()
 def restore_activations(checkpoint: ActivationCheckpoint, *, out: Optional[Tensor] = None) -> Tensor:
     """The matrix that a checkpoint stands for, in the type it was made from."""
     _check_checkpoint(checkpoint)
     codes, exponents, dtype = checkpoint
     rows, columns = codes.shape
-    tensors = {"codes": codes, "exponents": exponents}
     if out is not None:
-        _check_out(out, (rows, columns), (dtype,), **tensors)
-        tensors["out"] = out
-    _check_together(codes.device, **tensors)
+        _check_out(out, (rows, columns), (dtype,), codes=codes, exponents=exponents)
+    index = codes.get_device()
+    if index < 0 or exponents.get_device() != index or (out is not None and out.get_device() != index):
+        _refuse_devices(codes.device, codes=codes, exponents=exponents, out=out)
     if out is None:
         out = torch.empty((rows, columns), dtype=dtype, device=codes.device)
-    if out.numel():
-        with torch.cuda.device(codes.device):
-            native_call("soapmi_restore_activations", _DTYPES[dtype], codes.data_ptr(), _row_stride(codes),
-                        exponents.data_ptr(), _row_stride(exponents), rows, columns, out.data_ptr(), _row_stride(out),
-                        stream_of(codes))
+    if rows and columns:
+        _launch(index, "soapmi_restore_activations", _DTYPES[dtype], codes.data_ptr(), _row_stride(codes),
+                exponents.data_ptr(), _row_stride(exponents), rows, columns, out.data_ptr(), _row_stride(out))
     return out
 
 
 # ---- 8-bit integer product -----------------------------------------------------------------
 
 
-@torch.no_grad()
 def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
     """Codes (int8) and scales (float32, one for each row) of a matrix: scale = largest magnitude / 127,
     code = x / scale rounded to the nearest even.  The rows are tokens, or a weight's output channels.
     A row of zeros has scale 0; one that holds an infinity or NaN has scale NaN."""
-    _check_values("x", x)
-    require_device_tensor("x", x)
+    code = _check_values("x", x)
+    index = x.get_device()
+    if index < 0:
+        _refuse_devices(x.device, x=x)
     rows, columns = x.shape
     codes = _code_matrix(rows, columns, x.device)
     scales = torch.empty(rows, dtype=torch.float32, device=x.device)
     if rows:
-        with torch.cuda.device(x.device):
-            values, ldx = _rows(x)
-            native_call("soapmi_quantize_rows", _DTYPES[x.dtype], values.data_ptr(), ldx, rows, columns, codes.data_ptr(),
-                        _row_stride(codes), scales.data_ptr(), stream_of(x))
+        values, ldx = _rows(x)
+        _launch(index, "soapmi_quantize_rows", code, values.data_ptr(), ldx, rows, columns, codes.data_ptr(),
+                _row_stride(codes), scales.data_ptr())
     return codes, scales
 
 
@@ -396,13 +405,13 @@ def _check_codes(name: str, codes: Tensor, scales: Tensor) -> None:
     _check_matrix(f"{name}' scales", scales, 1)
     if scales.dtype != torch.float32:
         raise ValueError(f"{name}' scales must use float32, got {scales.dtype}.")
-    if scales.numel() != codes.size(0):
-        raise ValueError(f"{name} have {codes.size(0)} rows and {scales.numel()} scales.")
-    if scales.numel() > 1 and scales.stride(0) != 1:
+    rows, count = codes.size(0), scales.numel()
+    if count != rows:
+        raise ValueError(f"{name} have {rows} rows and {count} scales.")
+    if count > 1 and scales.stride(0) != 1:
         raise ValueError(f"{name}' scales must be contiguous.")
 
 
-@torch.no_grad()
 def int8_product(
     codes: Tensor,
     scales: Tensor,
@@ -420,25 +429,28 @@ def int8_product(
     _check_codes("codes", codes, scales)
     _check_codes("weight_codes", weight_codes, weight_scales)
     tokens, inner = codes.shape
-    outputs = weight_codes.size(0)
-    if weight_codes.size(1) != inner:
-        raise ValueError(f"weight_codes have {weight_codes.size(1)} columns, expected {inner}.")
+    outputs, width = weight_codes.shape
+    if width != inner:
+        raise ValueError(f"weight_codes have {width} columns, expected {inner}.")
     if inner > _INT8_MAX_INNER:
         raise ValueError(f"codes have {inner} columns, at most {_INT8_MAX_INNER} keep the integer sums inside 32 bits.")
-    tensors = {"codes": codes, "scales": scales, "weight_codes": weight_codes, "weight_scales": weight_scales}
     if out is not None:
-        _check_out(out, (tokens, outputs), tuple(_DTYPES), **tensors)
-        tensors["out"] = out
-    elif out_dtype not in _DTYPES:
-        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}.")
-    _check_together(codes.device, **tensors)
+        out_code = _check_out(out, (tokens, outputs), tuple(_DTYPES), codes=codes, scales=scales, weight_codes=weight_codes,
+                              weight_scales=weight_scales)
+    else:
+        out_code = _DTYPES.get(out_dtype)
+        if out_code is None:
+            raise ValueError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}.")
+    index = codes.get_device()
+    if (index < 0 or scales.get_device() != index or weight_codes.get_device() != index
+            or weight_scales.get_device() != index or (out is not None and out.get_device() != index)):
+        _refuse_devices(codes.device, codes=codes, scales=scales, weight_codes=weight_codes, weight_scales=weight_scales,
+                        out=out)
     if out is None:
         out = torch.empty((tokens, outputs), dtype=out_dtype, device=codes.device)
-    if out.numel():
-        with torch.cuda.device(codes.device):
-            rows, ldq = _rows(codes)
-            matrix, ldw = _rows(weight_codes)
-            native_call("soapmi_int8_product", rows.data_ptr(), ldq, scales.data_ptr(), matrix.data_ptr(), ldw,
-                        weight_scales.data_ptr(), tokens, outputs, inner, _DTYPES[out.dtype], out.data_ptr(),
-                        _row_stride(out), stream_of(codes))
+    if tokens and outputs:
+        rows, ldq = _rows(codes)
+        matrix, ldw = _rows(weight_codes)
+        _launch(index, "soapmi_int8_product", rows.data_ptr(), ldq, scales.data_ptr(), matrix.data_ptr(), ldw,
+                weight_scales.data_ptr(), tokens, outputs, inner, out_code, out.data_ptr(), _row_stride(out))
     return out
