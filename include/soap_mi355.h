@@ -194,8 +194,8 @@ int soapmi_col_major_to_row_major_f32(const float* in, int64_t ldi, float* out, 
  * their gradients are tokens, sorted by expert: expert e has the rows ends[e-1] .. ends[e]-1 (0 before
  * the first), `ends` being `experts` ascending int64 values on the device, at most `tokens`; it may be
  * NULL for one expert that has every row.  An expert may have no row.  Sizes stay on the device: no
- * call synchronises, needs a workspace or depends on where the rows are cut, and all of them can be
- * captured into a graph and replayed with other values in `ends`.  Values of `ends` that are not
+ * call synchronises or depends on where the rows are cut, and all of them can be captured
+ * into a graph and replayed with other values in `ends`.  Values of `ends` that are not
  * ascending or not in 0 .. tokens are held to that range, so every access stays inside the buffers,
  * but which rows are then computed is not specified.  A weight matrix is n x k (outputs x inputs);
  * expert e's starts e * stride elements after the first.  `dtype` and `out_dtype` are one of the
@@ -215,18 +215,24 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
                           int out_dtype, void* y, int64_t ldy, int zero_rest, void* stream);
 
 /* dW_e (n x k) = sum over e's rows t of gradient[t, :]^T x[t, :]; zeros for an expert without rows.
- * gradient: tokens x n, x: tokens x k, both of `dtype`; out_dtype is dtype or SOAPMI_FLOAT32. */
+ * gradient: tokens x n, x: tokens x k, both of `dtype`; out_dtype is dtype or SOAPMI_FLOAT32.
+ * Where few tiles have long sums these are cut into parts, which are added in order; that takes a
+ * workspace of soapmi_expert_weight_gradient_workspace_bytes (0: no use for one).  workspace may be NULL:
+ * the sums then stay whole (slower, and rounded in another order). */
 int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, const void* x, int64_t ldx,
                                   const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
-                                  int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* stream);
+                                  int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t tokens, int64_t n, int64_t k);
 
 /* The same with x as soapmi_checkpoint_activations saved it from values of `dtype` (16-bit types only: a
  * fp32 checkpoint is restored first).  The codes' steps are powers of two, so x enters the product
- * exactly as it is restored. */
+ * exactly as it is restored.  Where ldq is a multiple of 8, codes behind a row's last one, up to the next
+ * multiple of 8, may be read (every row, the last one too, has ldq of them). */
 int soapmi_expert_weight_gradient_saved(int dtype, const void* gradient, int64_t ldg, const int8_t* codes, int64_t ldq,
                                         const uint8_t* exponents, int64_t lde, const int64_t* ends, int64_t experts,
                                         int64_t tokens, int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw,
-                                        int64_t stride_dw, void* stream);
+                                        int64_t stride_dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Activation checkpoint of a rows x cols matrix: 8-bit codes (rows x cols) and an exponent for each row
  * and 128 columns (rows x ceil(cols / 128)).  With 2^(p-1) <= m < 2^p the largest magnitude of those

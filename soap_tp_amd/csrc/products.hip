@@ -13,6 +13,25 @@ extern template int row_products<ElemF16, XC>(hipStream_t, const RowProblem&, bo
 extern template int row_products<ElemI8, KC>(hipStream_t, const RowProblem&, bool);
 extern template int sum_products<ElemBF16>(hipStream_t, const SumProblem&, bool, bool);
 extern template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool, bool);
+
+// The parts' sums, added in order.
+static __global__ __launch_bounds__(256) void join_parts_kernel(SumProblem p) {
+  const int64_t matrix = (int64_t)p.rows * p.cols, all = matrix * p.groups.experts;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= all) return;
+  float sum = p.partials[at];
+  for (int part = 1; part < p.parts; ++part) sum += p.partials[part * all + at];
+  const int64_t e = at / matrix, in = at - e * matrix;
+  const int64_t r = in / p.cols, c = in - r * p.cols;
+  store_value(p.d, e * p.stride_d + r * p.ldd + c, p.out_type, sum);
+}
+
+int launch_join(hipStream_t stream, const SumProblem& p) {
+  const int64_t all = (int64_t)p.groups.experts * p.rows * p.cols;  // (at most 128 tiles)
+  hipLaunchKernelGGL(join_parts_kernel, dim3((unsigned)ceil_div64(all, 256)), dim3(256), 0, stream, p);
+  SOAPMI_LAUNCH_CHECK();
+  return kOk;
+}
 }  // namespace soapmi
 
 using namespace soapmi;
@@ -59,19 +78,11 @@ int launch_rows_f32(hipStream_t stream, RowProblem p, int k_contiguous, int vec_
 
 template <class Cfg>
 int launch_sums_f32(hipStream_t stream, SumProblem p, int vec_dy, int vec_x) {
-  p.tiles_r = (int)ceil_div64(p.rows, Cfg::BN);
-  p.tiles_c = (int)ceil_div64(p.cols, Cfg::BM);
-  const int64_t chunk = ((int64_t)p.tiles_r * p.tiles_c + 7) / 8;
   unsigned grid;
-  if (int rc = grid_of(8 * chunk * p.groups.experts, &grid)) return rc;
+  if (int rc = sum_grid(p, Cfg::BN, Cfg::BM, &grid)) return rc;
   hipLaunchKernelGGL((sum_product_f32_kernel<Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p, vec_dy, vec_x);
   SOAPMI_LAUNCH_CHECK();
-  return kOk;
-}
-
-bool wide_stores(const void* base, int64_t ld, int64_t stride, int out_dtype) {
-  const int64_t bytes = value_bytes(out_dtype);
-  return aligned16(base) && ld * bytes % 16 == 0 && stride * bytes % 16 == 0;
+  return p.parts > 1 ? launch_join(stream, p) : kOk;
 }
 
 int check_gradient(int dtype, int out_dtype, const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
@@ -84,8 +95,10 @@ int check_gradient(int dtype, int out_dtype, const int64_t* ends, int64_t expert
   return kOk;
 }
 
-SumProblem sum_problem(int dtype, const void* gradient, int64_t ldg, const int64_t* ends, int64_t experts, int64_t tokens,
-                       int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw, int64_t stride_dw) {
+// With a workspace for them, long sums for few tiles are cut into parts.
+int sum_problem(int dtype, const void* gradient, int64_t ldg, const int64_t* ends, int64_t experts, int64_t tokens, int64_t n,
+                int64_t k, int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* workspace, size_t workspace_bytes,
+                SumProblem* out) {
   SumProblem p = {};
   p.groups = RowGroups{ends, (int)experts, 0, (int)tokens};
   p.r = static_cast<const char*>(gradient);
@@ -96,8 +109,19 @@ SumProblem sum_problem(int dtype, const void* gradient, int64_t ldg, const int64
   p.ldd = lddw;
   p.stride_d = stride_dw;
   p.out_type = out_dtype;
-  p.wide = wide_stores(dw, lddw, experts > 1 ? stride_dw : 0, out_dtype);
-  return p;
+  p.parts = 1;
+  const size_t need = sum_partials_bytes(experts, tokens, n, k);
+  if (workspace && need) {
+    if (workspace_bytes < need) {
+      set_error("workspace holds %zu bytes, %zu are required", workspace_bytes, need);
+      return kWorkspaceTooSmall;
+    }
+    SOAPMI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, "workspace must be aligned to 4 bytes");
+    p.parts = sum_parts(experts, tokens, n, k);
+    p.partials = static_cast<float*>(workspace);
+  }
+  *out = p;
+  return kOk;
 }
 
 template <class T>
@@ -182,7 +206,6 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
   p.y = y;
   p.ldy = ldy;
   p.out_type = out_dtype;
-  p.wide = wide_stores(y, ldy, 0, out_dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == kFloat32) {
     // (contiguous along: weights k, x the inner extent)
@@ -201,11 +224,15 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
 
 int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, const void* x, int64_t ldx,
                                   const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
-                                  int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* stream) {
+                                  int out_dtype, void* dw, int64_t lddw, int64_t stride_dw, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   if (int rc = check_gradient(dtype, out_dtype, ends, experts, tokens, n, k, ldg, ldx, lddw, stride_dw)) return rc;
   if (experts == 0 || n == 0 || k == 0) return kOk;
   SOAPMI_REQUIRE(dw && (tokens == 0 || (gradient && x)), "buffer addresses must be nonzero");
-  SumProblem p = sum_problem(dtype, gradient, ldg, ends, experts, tokens, n, k, out_dtype, dw, lddw, stride_dw);
+  SumProblem p;
+  if (int rc = sum_problem(dtype, gradient, ldg, ends, experts, tokens, n, k, out_dtype, dw, lddw, stride_dw, workspace,
+                           workspace_bytes, &p))
+    return rc;
   p.c = static_cast<const char*>(x);
   p.ldc = ldx * value_bytes(dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -222,20 +249,27 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
 int soapmi_expert_weight_gradient_saved(int dtype, const void* gradient, int64_t ldg, const int8_t* codes, int64_t ldq,
                                         const uint8_t* exponents, int64_t lde, const int64_t* ends, int64_t experts,
                                         int64_t tokens, int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw,
-                                        int64_t stride_dw, void* stream) {
+                                        int64_t stride_dw, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_gradient(dtype, out_dtype, ends, experts, tokens, n, k, ldg, ldq, lddw, stride_dw)) return rc;
   SOAPMI_REQUIRE(dtype != kFloat32, "dtype must be 1 (bfloat16) or 2 (float16): restore a float32 checkpoint first");
   SOAPMI_REQUIRE(lde >= ceil_div64(k, kCheckpointBlock), "leading dimensions are too small");
   if (experts == 0 || n == 0 || k == 0) return kOk;
   SOAPMI_REQUIRE(dw && (tokens == 0 || (gradient && codes && exponents)), "buffer addresses must be nonzero");
-  SumProblem p = sum_problem(dtype, gradient, ldg, ends, experts, tokens, n, k, out_dtype, dw, lddw, stride_dw);
+  SumProblem p;
+  if (int rc = sum_problem(dtype, gradient, ldg, ends, experts, tokens, n, k, out_dtype, dw, lddw, stride_dw, workspace,
+                           workspace_bytes, &p))
+    return rc;
   p.c = reinterpret_cast<const char*>(codes);
   p.ldc = ldq;
   p.exponents = exponents;
   p.ld_exp = lde;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool direct = direct_ok(gradient, p.ldr, n * 2, 64);
+  const bool direct = direct_ok(gradient, p.ldr, n * 2, 64) && reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
   return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct, true) : sum_products<ElemF16>(s, p, direct, true);
+}
+
+size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t tokens, int64_t n, int64_t k) {
+  return experts > 0 && tokens > 0 && n > 0 && k > 0 ? sum_partials_bytes(experts, tokens, n, k) : 0;
 }
 
 int soapmi_checkpoint_activations(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes,
@@ -290,7 +324,6 @@ int soapmi_int8_product(const int8_t* codes, int64_t ldq, const float* scales, c
   p.y = y;
   p.ldy = ldy;
   p.out_type = out_dtype;
-  p.wide = wide_stores(y, ldy, 0, out_dtype);
   p.token_scale = scales;
   p.channel_scale = w_scales;
   const bool direct = direct_ok(codes, ldq, k, 256) && direct_ok(w_codes, ldw, k, 256);

@@ -102,33 +102,51 @@ struct RowTile {
 // tiles, walked in groups of up to 8 row tiles by all columns, so that a weight tile is fetched into
 // that XCD's L2 once for its row tiles.  Returns false behind the last tile.
 template <int BR, int GRAIN>
-__device__ __forceinline__ bool locate_rows(const RowGroups& g, int tiles_c, int wg, RowTile& tile, int& tile_c) {
+__device__ __forceinline__ bool locate_rows(const RowGroups& g, unsigned tiles_c, unsigned wg, RowTile& tile, int& tile_c) {
   const int lane = threadIdx.x & 63;
   const int groups = g.experts + g.rest;
   int total = 0;
   int first_tiles = 0, first_begin = 0, first_end = 0;  // of the first 64 groups, kept for the search
-  for (int e0 = 0; e0 < groups; e0 += 64) {
-    int begin = 0, end = 0;
-    if (e0 + lane < groups) group_rows(g, e0 + lane, begin, end);
-    const int tiles = wave_inclusive_sum((end - begin + BR - 1) / BR, lane);
-    if (e0 == 0) {
-      first_tiles = tiles;
-      first_begin = begin;
-      first_end = end;
+  if (g.ends == nullptr) {
+    total = (g.tokens + BR - 1) / BR;
+  } else {
+    for (int e0 = 0; e0 < groups; e0 += 64) {
+      int begin = 0, end = 0;
+      if (e0 + lane < groups) group_rows(g, e0 + lane, begin, end);
+      const int tiles = wave_inclusive_sum((end - begin + BR - 1) / BR, lane);
+      if (e0 == 0) {
+        first_tiles = tiles;
+        first_begin = begin;
+        first_end = end;
+      }
+      total += __builtin_amdgcn_readlane(tiles, 63);
     }
-    total += __shfl(tiles, 63);
   }
-  total = __builtin_amdgcn_readfirstlane(total);
-  const int64_t all = (int64_t)total * tiles_c;
-  const int64_t chunk = (all + 7) >> 3;
-  const int64_t t = (int64_t)(wg & 7) * chunk + (wg >> 3);
+  // (32-bit numbers throughout: a launch has fewer than 2^31 tiles, and divisions of 64-bit ones are long)
+  const unsigned all = (unsigned)total * tiles_c;
+  const unsigned chunk = (all + 7) >> 3;
+  const unsigned t = (wg & 7) * chunk + (wg >> 3);
   if ((wg >> 3) >= chunk || t >= all) return false;
-  constexpr int GR = 8;
-  const int64_t per = (int64_t)GR * tiles_c;
-  const int band = (int)(t / per), in_band = (int)(t - band * per);
-  const int rows = min(GR, total - band * GR);
-  const int tr = band * GR + in_band % rows;
-  tile_c = in_band / rows;
+  constexpr unsigned GR = 8;
+  const unsigned per = GR * tiles_c;
+  const unsigned band = t / per, in_band = t - band * per;
+  const unsigned rows = min(GR, (unsigned)total - band * GR);
+  const unsigned column = in_band / rows;
+  const int tr = (int)(band * GR + in_band - column * rows);
+  tile_c = __builtin_amdgcn_readfirstlane((int)column);
+  auto found = [&](int expert, int begin, int end, int nth) {
+    const unsigned grains = (unsigned)(end - begin + GRAIN - 1) / GRAIN, share = (unsigned)(end - begin + BR - 1) / BR;
+    const unsigned each = grains / share, larger = grains - each * share;  // the first `larger` tiles have one more
+    const int first = (int)(nth * each + min((unsigned)nth, larger)) * GRAIN;
+    const int last = min(end - begin, first + (int)(each + ((unsigned)nth < larger ? 1 : 0)) * GRAIN);
+    tile.expert = __builtin_amdgcn_readfirstlane(expert);
+    tile.row = __builtin_amdgcn_readfirstlane(begin + first);
+    tile.rows = __builtin_amdgcn_readfirstlane(last - first);
+  };
+  if (g.ends == nullptr) {
+    found(0, 0, g.tokens, tr);
+    return true;
+  }
   int before = 0;
   for (int e0 = 0; e0 < groups; e0 += 64) {
     int begin = first_begin, end = first_end, tiles = first_tiles;
@@ -139,20 +157,12 @@ __device__ __forceinline__ bool locate_rows(const RowGroups& g, int tiles_c, int
     }
     const uint64_t behind = __ballot(before + tiles > tr);
     if (behind) {
-      const int at = __ffsll((unsigned long long)behind) - 1;
-      const int up_to = at ? __shfl(tiles, at - 1) : 0;
-      begin = __shfl(begin, at);
-      end = __shfl(end, at);
-      const int count = end - begin, share = (count + BR - 1) / BR, nth = tr - before - up_to;
-      const int64_t grains = (count + GRAIN - 1) / GRAIN;
-      const int first = (int)(nth * grains / share) * GRAIN;
-      const int last = min(count, (int)((nth + 1) * grains / share) * GRAIN);
-      tile.expert = __builtin_amdgcn_readfirstlane(e0 + at);
-      tile.row = __builtin_amdgcn_readfirstlane(begin + first);
-      tile.rows = __builtin_amdgcn_readfirstlane(last - first);
+      const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)behind) - 1);
+      const int up_to = at ? __builtin_amdgcn_readlane(tiles, at - 1) : 0;
+      found(e0 + at, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), tr - before - up_to);
       return true;
     }
-    before += __shfl(tiles, 63);
+    before += __builtin_amdgcn_readlane(tiles, 63);
   }
   return false;  // (not reached: tr < total)
 }
@@ -177,8 +187,9 @@ __device__ __forceinline__ int column_of(int i, int m) { return 32 * (i >> 1) + 
 enum Layout { KC, XC };
 // How an operand gets to LDS.  Direct: 16-byte pieces straight from memory (aligned operands).  Staged:
 // through registers, any alignment and size.  Codes: through registers, 8-bit codes of an activation
-// checkpoint expanded to 16-bit values on the way.
-enum Source { Direct, Staged, Codes };
+// checkpoint expanded to 16-bit values on the way, rows of whole, aligned pieces.  AnyCodes: codes of any
+// alignment and size.
+enum Source { Direct, Staged, Codes, AnyCodes };
 
 struct Operand {
   const char* base;  // tile's first element
@@ -203,9 +214,6 @@ __device__ __forceinline__ void load_to_lds(i32x4 resource, unsigned offset, uns
                : "s"(lds), "v"(offset), "s"(resource), "s"(more)
                : "memory", "m0");
 }
-// Every load to LDS and every LDS access that this wavefront has started is done, and so is every other
-// wavefront's of the workgroup.
-__device__ __forceinline__ void wait_arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ i32x4 buffer_of(const char* base, int bytes) {
   const uint64_t address = reinterpret_cast<uint64_t>(base);
@@ -241,21 +249,22 @@ __device__ __forceinline__ float exponent_value(int code) {  // 2^(code - 127); 
 }
 
 // One operand of a tile: BX rows (or columns), slabs of 128 bytes (KC) or 64 values (XC) of k.
-template <class E, Layout L, Source S, int BX, int NT, bool COLUMN>
+template <class E, Layout L, Source S, int BX, int NT, bool COLUMN, int AHEAD>
 struct Loader {
   static constexpr int SLAB_K = L == KC ? 128 / E::SIZE : 64;
   static constexpr int BYTES = L == KC ? BX * 128 : 64 * BX * E::SIZE;
   static constexpr int PIECES = BYTES / 16;
   static constexpr int NP = (PIECES + NT - 1) / NT;
   static_assert(L == KC || E::SIZE == 2, "transposing reads are of 16-bit values");
-  static_assert(S != Codes || L == XC, "codes are expanded along x");
+  static constexpr bool CODES = S == Codes || S == AnyCodes;
+  static_assert(!CODES || L == XC, "codes are expanded along x");
   static_assert(S != Direct || PIECES % 64 == 0, "whole wavefronts fetch");
   static constexpr int PER_ROW = L == KC ? 8 : BX * E::SIZE / 16;  // pieces in an LDS row
 
   // Piece q = tid + i * NT of an operand lies i * STEP stored rows below piece tid and in the same place of
   // its row, since the permutations look at row bits below STEP only.
   static constexpr int STEP = NT / PER_ROW;
-  static_assert(S != Direct || NP == 1 || STEP % 16 == 0, "one offset serves all of a lane's pieces");
+  static_assert(NP == 1 || STEP % 16 == 0, "one place in the row serves all of a lane's pieces");
 
   const char* base;
   int64_t ld;
@@ -264,11 +273,11 @@ struct Loader {
   int64_t ld_exp;
   int tid;
   unsigned offset, offset_now;  // Direct: of the lane's first piece; in the slab being sent
-  int first_piece;
+  int first_row, first_piece;   // of the lane's first piece
   i32x4 resource;
   struct Two { unsigned w[2]; };
-  std::conditional_t<S == Codes, Two, i32x4> held[S == Direct ? 1 : NP];
-  int held_exp[S == Codes ? NP : 1];
+  std::conditional_t<CODES, Two, i32x4> held[S == Direct ? 1 : AHEAD][S == Direct ? 1 : NP];  // slabs in registers
+  int held_exp[CODES ? AHEAD : 1][CODES ? NP : 1];
 
   // stored row and piece of LDS piece q
   static __device__ __forceinline__ void place(int q, int& row, int& piece) {
@@ -285,10 +294,9 @@ struct Loader {
     exponents = o.exponents;
     ld_exp = o.ld_exp;
     tid = tid_;
+    place(tid, first_row, first_piece);
     if constexpr (S == Direct) {
-      int row;
-      place(tid, row, first_piece);
-      offset = (unsigned)(row * (int)ld + first_piece * 16);
+      offset = (unsigned)(first_row * (int)ld + first_piece * 16);
       if (L == XC && first_piece * 16 >= valid * E::SIZE) offset = kOutside;
     }
   }
@@ -311,59 +319,66 @@ struct Loader {
     load_to_lds(resource, offset_now, (unsigned)(i * STEP * (int)ld), lds + wave * 1024 + i * NT * 16);
   }
 
-  // Staged and Codes: a lane's first COUNT pieces of slab kt come to registers.
-  template <int COUNT>
-  __device__ __forceinline__ void fetch(int kt, int k_left) {
-    const char* at = slab(kt);
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      const int q = tid + i * NT;
-      if (PIECES % NT != 0 && q >= PIECES) break;
-      int row, piece;
-      place(q, row, piece);
+  // Other sources: piece i of slab kt comes to register set `set`.  k_left as for aim().
+  __device__ __forceinline__ void fetch(int i, int kt, int k_left, int set) {
+    if constexpr (S != Direct) {
+      if (PIECES % NT != 0 && tid + i * NT >= PIECES) return;
+      const int row = first_row + i * STEP;
       if constexpr (S == Staged) {
+        const char* at = slab(kt) + first_piece * 16;
         if (L == KC) {
           const int r = min(row, valid - 1);  // rows behind the last one only reach results that are not stored
-          held[i] = load_bytes(at + r * ld + piece * 16, k_left * E::SIZE - piece * 16);
+          at += r * ld;
+          if (k_left >= SLAB_K) held[set][i] = load_bytes(at, 16);
+          else held[set][i] = load_bytes(at, k_left * E::SIZE - first_piece * 16);
         } else {
-          held[i] = row < k_left ? load_bytes(at + row * ld + piece * 16, valid * E::SIZE - piece * 16) : i32x4{0, 0, 0, 0};
+          at += row * ld;
+          if (k_left >= SLAB_K && valid == BX) held[set][i] = load_bytes(at, 16);
+          else held[set][i] = load_bytes(at, row < k_left ? valid * E::SIZE - first_piece * 16 : 0);
         }
       } else if constexpr (S == Codes) {
-        // eight codes for a piece of eight 16-bit values
-        const int count = row < k_left ? valid - piece * 8 : 0;
-        held[i] = Two{};
-        held_exp[i] = 0;
+        // eight codes for a piece of eight 16-bit values; a row behind the last one is the slab's first with
+        // step zero, a slab behind the last one the first slab, and columns behind the last one are whatever
+        // stands there: they only reach results that are not stored
+        const bool inside = row < k_left;
+        const int kt_inside = k_left > 0 ? kt : 0;
+        const char* at = slab(kt_inside) + (first_piece * 8 < valid ? first_piece * 8 : 0);
+        const uint8_t* steps = exponents + (int64_t)kt_inside * 64 * ld_exp + (first_piece * 8 < valid ? first_piece >> 4 : 0);
+        const int r = inside ? row : 0;
+        const unsigned e = steps[r * ld_exp];
+        __builtin_memcpy(&held[set][i], __builtin_assume_aligned(at + r * ld, 8), 8);
+        held_exp[set][i] = inside ? e : 0;
+      } else {
+        const int count = row < k_left ? valid - first_piece * 8 : 0;
+        held[set][i] = Two{};
+        held_exp[set][i] = 0;
         if (count > 0) {
-          const char* p = at + row * ld + piece * 8;
-          held_exp[i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (piece >> 4)];
-          if (count >= 8) {
-            __builtin_memcpy(&held[i], p, 8);
-          } else {
-            char b[8];
+          const char* p = slab(kt) + row * ld + first_piece * 8;
+          held_exp[set][i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (first_piece >> 4)];
+          char b[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
-            __builtin_memcpy(&held[i], b, 8);
-          }
+          for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
+          __builtin_memcpy(&held[set][i], b, 8);
         }
       }
     }
   }
 
-  // ... and piece i of it goes on to LDS.
-  __device__ __forceinline__ void put(int i, char* lds) {
+  // ... and goes on to LDS.
+  __device__ __forceinline__ void put(int i, int set, char* lds) {
     const int q = tid + i * NT;
     if constexpr (S != Direct) {
       if (PIECES % NT == 0 || q < PIECES) {
         if constexpr (S == Staged) {
-          *reinterpret_cast<i32x4*>(lds + q * 16) = held[i];
+          *reinterpret_cast<i32x4*>(lds + q * 16) = held[set][i];
         } else {
           // code * 2^e is exact in bf16 (8 bits of mantissa) and, with the exponents that
           // checkpoints of fp16 values have, in fp16
-          const float step = exponent_value(held_exp[i]);
+          const float step = exponent_value(held_exp[set][i]);
           typename E::Scalar v[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            v[j] = (typename E::Scalar)((float)(int8_t)(held[i].w[j >> 2] >> (8 * (j & 3))) * step);
+            v[j] = (typename E::Scalar)((float)(int8_t)(held[set][i].w[j >> 2] >> (8 * (j & 3))) * step);
           __builtin_memcpy(lds + q * 16, v, 16);
         }
       }
@@ -396,9 +411,11 @@ struct Loader {
   }
 };
 
-template <int BR_, int BC_, int WR_, int WC_>
+// BR x BC results, WR x WC wavefronts.  STAGES slabs are in LDS or on their way there (Direct operands;
+// with others two, and AHEAD more in registers).
+template <int BR_, int BC_, int WR_, int WC_, int STAGES_, int AHEAD_>
 struct ProductTile {
-  static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_;
+  static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, STAGES = STAGES_, AHEAD = AHEAD_;
   static constexpr int NT = 64 * WR * WC;
   static constexpr int TR = BR / WR / 16, TC = BC / WC / 16;
   static_assert(TC % 2 == 0, "columns are dealt to pairs of fragments");
@@ -410,17 +427,23 @@ struct ProductTile {
 // takes all of them for a shorter time.
 //
 // A slab is two steps of the matrix instruction's k.  While a wavefront multiplies one step's fragments,
-// the next step's come from LDS into other registers, and two slabs are in LDS or on their way.  What
+// the next step's come from LDS into other registers, and further slabs are in LDS or on their way.  What
 // moves data is dealt out between the rows of matrix instructions: a wavefront issues in order, and the
 // loads of a whole slab in a row would keep it from issuing anything else for as long as they take.
 template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg, int A = Cfg::TR>
 struct TileProduct {
-  using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false>;
-  using LoadC = Loader<E, LC, SC, Cfg::BC, Cfg::NT, true>;
+  static constexpr bool DIRECT = SR == Direct && SC == Direct;
+  static constexpr int STAGES = DIRECT ? Cfg::STAGES : 2, AHEAD = DIRECT ? 1 : Cfg::AHEAD;
+  static_assert((STAGES & (STAGES - 1)) == 0, "a slab's stage is its number's low bits");
+  using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false, AHEAD>;
+  using LoadC = Loader<E, LC, SC, Cfg::BC, Cfg::NT, true, AHEAD>;
   static constexpr int SLAB_K = LoadR::SLAB_K;
   static_assert(LoadR::SLAB_K == LoadC::SLAB_K, "one slab for both operands");
+  static_assert(!DIRECT || STAGES == 2 || (LoadR::PIECES % Cfg::NT == 0 && LoadC::PIECES % Cfg::NT == 0),
+                "waiting by count: every lane has the same number of loads");
   static constexpr int STAGE = LoadR::BYTES + LoadC::BYTES;
-  static constexpr int LDS_BYTES = 2 * STAGE;
+  static constexpr int LDS_BYTES = STAGES * STAGE;
+  static_assert(LDS_BYTES >= 8192 * Cfg::NT / 64, "results pass through it (kStoreBytes)");
   static constexpr int TR = A, TC = Cfg::TC, READS = TR + TC;
   // pieces that a lane moves per slab: of a KC row operand only those of the rows that are computed
   static constexpr int PIECES_R = LR == KC ? (A * Cfg::WR * 16 + LoadR::STEP - 1) / LoadR::STEP : LoadR::NP;
@@ -454,41 +477,46 @@ struct TileProduct {
     LoadC lc;
     lr.init(r, tid);
     lc.init(c, tid);
+    auto stage_of = [](int kt) { return (kt & (STAGES - 1)) * STAGE; };
     auto aim = [&](int kt) {
       if constexpr (SR == Direct) lr.aim(kt, k_count - kt * SLAB_K);
       if constexpr (SC == Direct) lc.aim(kt, k_count - kt * SLAB_K);
     };
-    auto fetch = [&](int kt) {
-      if constexpr (SR != Direct) lr.template fetch<PIECES_R>(kt, k_count - kt * SLAB_K);
-      if constexpr (SC != Direct) lc.template fetch<LoadC::NP>(kt, k_count - kt * SLAB_K);
+    // piece n of slab kt: to registers (operands that are not Direct) ...
+    auto fetch = [&](int n, int kt, int set) {
+      if (n < PIECES_R) lr.fetch(n, kt, k_count - kt * SLAB_K, set);
+      else lc.fetch(n - PIECES_R, kt, k_count - kt * SLAB_K, set);
     };
-    // piece n of slab kt on its last way: sent from memory, or put from registers
-    auto move = [&](int n, int kt) {
-      const int stage = (kt & 1) * STAGE;
+    // ... and to LDS, from there or straight from memory
+    auto move = [&](int n, int kt, int set) {
       if (n < PIECES_R) {
-        if constexpr (SR == Direct) lr.send(n, lds_address + stage);
-        else lr.put(n, lds + stage);
+        if constexpr (SR == Direct) lr.send(n, lds_address + stage_of(kt));
+        else lr.put(n, set, lds + stage_of(kt));
       } else {
-        if constexpr (SC == Direct) lc.send(n - PIECES_R, lds_address + stage + LoadR::BYTES);
-        else lc.put(n - PIECES_R, lds + stage + LoadR::BYTES);
+        if constexpr (SC == Direct) lc.send(n - PIECES_R, lds_address + stage_of(kt) + LoadR::BYTES);
+        else lc.put(n - PIECES_R, set, lds + stage_of(kt) + LoadR::BYTES);
       }
     };
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-      if (kt < slabs) {
-        aim(kt);
-        fetch(kt);
+    for (int kt = 0; kt < STAGES; ++kt) {
+      aim(kt);
 #pragma unroll
-        for (int n = 0; n < PIECES; ++n) move(n, kt);
+      for (int n = 0; n < PIECES; ++n) {
+        fetch(n, kt, 0);
+        move(n, kt, 0);
       }
-    fetch(2);
-    wait_arrived();
+    }
+#pragma unroll
+    for (int set = 0; set < AHEAD; ++set)
+#pragma unroll
+      for (int n = 0; n < PIECES; ++n) fetch(n, STAGES + set, set);
+    arrive<(STAGES - 1) * PIECES>();
     Fragments f0, f1;
 #pragma unroll
     for (int n = 0; n < READS; ++n) read(f0, n, lds, wr0, wc0, 0, lane);
-    for (int kt = 0; kt + 1 < slabs; ++kt) {
-      const char* stage = lds + (kt & 1) * STAGE;
-      const char* next = lds + ((kt + 1) & 1) * STAGE;
+    auto slab = [&](int kt, int set) {
+      const char* stage = lds + stage_of(kt);
+      const char* next = lds + stage_of(kt + 1);
       // first step; the second one's fragments
 #pragma unroll
       for (int j = 0; j < TR; ++j) {
@@ -498,29 +526,51 @@ struct TileProduct {
         __builtin_amdgcn_sched_barrier(0);
       }
       // Every wavefront has read slab kt, and slab kt + 1 has arrived.
-      wait_arrived();
-      aim(kt + 2);
-      // second step; the next slab's first fragments, and the slab after that into the place of this one
+      arrive<(STAGES - 2) * PIECES>();
+      aim(kt + STAGES);
+      // second step; the next slab's first fragments, and a slab to come into the place of this one
       // (behind the last slab zeros, rather than a branch around every move)
 #pragma unroll
       for (int j = 0; j < TR; ++j) {
 #pragma unroll
         for (int n = j * READS / TR; n < (j + 1) * READS / TR; ++n) read(f0, n, next, wr0, wc0, 0, lane);
 #pragma unroll
-        for (int n = j * PIECES / TR; n < (j + 1) * PIECES / TR; ++n) move(n, kt + 2);
+        for (int n = j * PIECES / TR; n < (j + 1) * PIECES / TR; ++n) {
+          move(n, kt + STAGES, set);
+          fetch(n, kt + STAGES + AHEAD, set);
+        }
         multiply_row(f1, j, acc);
         __builtin_amdgcn_sched_barrier(0);
       }
-      fetch(kt + 3);
+    };
+    for (int kt = 0; kt + 1 < slabs; kt += AHEAD) {  // (register sets are numbered at compile time)
+#pragma unroll
+      for (int set = 0; set < AHEAD; ++set)
+        if (kt + set + 1 < slabs) slab(kt + set, set);
     }
-    const char* last = lds + ((slabs - 1) & 1) * STAGE;
+    const char* last = lds + stage_of(slabs - 1);
 #pragma unroll
     for (int n = 0; n < READS; ++n) read(f1, n, last, wr0, wc0, 1, lane);
 #pragma unroll
     for (int j = 0; j < TR; ++j) multiply_row(f0, j, acc);
 #pragma unroll
     for (int j = 0; j < TR; ++j) multiply_row(f1, j, acc);
+    wait_lds();
     wait_loads<0>();  // no load may write to LDS once the workgroup has given it back
+  }
+
+  // All but the last LATER loads to LDS of every wavefront, and all its LDS accesses, are done.
+  template <int LATER>
+  static __device__ __forceinline__ void arrive() {
+    if constexpr (DIRECT) wait_loads<LATER>();
+    else wait_loads_to_lds();
+    wait_lds();
+    barrier();
+  }
+  // With operands that pass through registers, the loads to LDS are not the only ones and cannot be
+  // counted from here: all are waited for (none, if no operand is Direct: LDS writes are waited for as such).
+  static __device__ __forceinline__ void wait_loads_to_lds() {
+    if constexpr (SR == Direct || SC == Direct) wait_loads<0>();
   }
 };
 
@@ -531,7 +581,6 @@ struct Result {
   int64_t ld;      // in elements
   int rows, cols;  // of the tile that exist
   int type;        // kFloat32, kBFloat16, kFloat16
-  int wide;        // 16-byte (16-bit: 8 values) stores are legal
 };
 
 __device__ __forceinline__ void store_value(void* base, int64_t at, int type, float v) {
@@ -540,58 +589,106 @@ __device__ __forceinline__ void store_value(void* base, int64_t at, int type, fl
   else static_cast<_Float16*>(base)[at] = (_Float16)v;
 }
 
+// Eight consecutive values, at any address (memory takes 16 bytes anywhere).
 template <class Scalar>
 __device__ __forceinline__ void store_eight(void* base, int64_t at, const float (&v)[8]) {
   Scalar out[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) out[q] = (Scalar)v[q];
-  constexpr int N = sizeof(out) / 16;
-  i32x4 piece[N];
-  __builtin_memcpy(piece, out, sizeof(out));
-#pragma unroll
-  for (int q = 0; q < N; ++q) reinterpret_cast<i32x4*>(static_cast<Scalar*>(base) + at)[q] = piece[q];
+  __builtin_memcpy(static_cast<Scalar*>(base) + at, out, sizeof(out));
 }
 
-// scale: (row of tile, column of tile, accumulator) -> result.
-template <class Cfg, int A, class Acc, class Scale>
-__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[A][Cfg::TC], const Scale& scale) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m = lane & 15, g = lane >> 4;
-  const int wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
-#pragma unroll
-  for (int j = 0; j < A; ++j) {
-    const int r = (Cfg::WR * j + wave % Cfg::WR) * 16 + m;
-    if (r >= o.rows) continue;
-#pragma unroll
-    for (int i = 0; i < Cfg::TC; i += 2) {
-      const int c = wc0 + 32 * (i >> 1) + 8 * g;
-      if (c >= o.cols) continue;
-      float v[8];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = scale(r, min(c + q, o.cols - 1), acc[j][i + (q >> 2)][q & 3]);
-      const int64_t at = (int64_t)r * o.ld + c;
-      if (o.wide && c + 8 <= o.cols) {
-        if (o.type == kFloat32) store_eight<float>(o.base, at, v);
-        else if (o.type == kBFloat16) store_eight<__bf16>(o.base, at, v);
-        else store_eight<_Float16>(o.base, at, v);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (c + q < o.cols) store_value(o.base, at + q, o.type, v[q]);
-      }
-    }
-  }
-}
-
+// What an accumulator is multiplied by: for a lane's columns, read once, and for a row.
 struct Unscaled {
-  __device__ __forceinline__ float operator()(int, int, float v) const { return v; }
+  template <int TC>
+  struct Columns {
+    __device__ __forceinline__ Columns(const Unscaled&, int, int) {}
+    __device__ __forceinline__ float operator()(int, int, float, float v) const { return v; }
+  };
+  __device__ __forceinline__ float row(int) const { return 1.0f; }
 };
 // The integer sum is exact; it is rounded to fp32 once, then scaled by the token and by the channel.
 struct TokenChannel {
   const float* token;
   const float* channel;
-  __device__ __forceinline__ float operator()(int r, int c, int v) const { return (float)v * token[r] * channel[c]; }
+  template <int TC>
+  struct Columns {
+    float channel[TC / 2][8];
+    __device__ __forceinline__ Columns(const TokenChannel& s, int c0, int cols) {  // columns c0 + 32 i .. + 7
+#pragma unroll
+      for (int i = 0; i < TC / 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) channel[i][q] = s.channel[min(c0 + 32 * i + q, cols - 1)];
+    }
+    __device__ __forceinline__ float operator()(int i, int q, float token, int v) const { return (float)v * token * channel[i][q]; }
+  };
+  __device__ __forceinline__ float row(int r) const { return token[r]; }
 };
+
+// A wavefront's results go through its share of LDS, so that it stores whole rows of its part of the tile
+// (64 bytes and more) instead of 16 bytes here and there.  Only its own accesses order these, no barrier.
+constexpr int kStoreBytes = 8192;  // of LDS for each wavefront
+
+template <class Cfg, class Out, int A, class Acc, class Scale>
+__device__ __forceinline__ void store_tile_as(const Result& o, const Acc (&acc)[A][Cfg::TC], const Scale& scale, char* lds) {
+  constexpr int WIDTH = Cfg::TC * 16 * (int)sizeof(Out), PIECES = WIDTH / 16;  // bytes and 16-byte pieces of a row
+  constexpr int FIT = kStoreBytes / (16 * WIDTH), AT_ONCE = FIT < A ? FIT : A;  // fragments of rows that fit
+  constexpr int VALUES = 16 / (int)sizeof(Out);
+  static_assert(FIT >= 1 && PIECES <= 64 && AT_ONCE * 16 * PIECES >= 64, "store layout");
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m = lane & 15, g = lane >> 4;
+  const int wr = wave % Cfg::WR, wc0 = (wave / Cfg::WR) * (Cfg::TC * 16);
+  char* mine = lds + wave * kStoreBytes;
+  const typename Scale::template Columns<Cfg::TC> columns(scale, wc0 + 8 * g, o.cols);
+#pragma unroll
+  for (int j0 = 0; j0 < A; j0 += AT_ONCE) {
+#pragma unroll
+    for (int jj = 0; jj < AT_ONCE; ++jj) {
+      if (j0 + jj >= A) continue;
+      const float row = scale.row(min((Cfg::WR * (j0 + jj) + wr) * 16 + m, o.rows - 1));
+#pragma unroll
+      for (int i = 0; i < Cfg::TC; i += 2) {
+        Out v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (Out)columns(i >> 1, q, row, acc[(j0 + jj) % A][i + (q >> 2)][q & 3]);
+#pragma unroll
+        for (int h = 0; h < 8 / VALUES; ++h) {
+          const int piece = (16 * i + 8 * g) / VALUES + h;
+          i32x4 w;
+          __builtin_memcpy(&w, v + h * VALUES, 16);
+          *reinterpret_cast<i32x4*>(mine + (jj * 16 + m) * WIDTH + ((piece ^ (m & (PIECES - 1) & 7)) << 4)) = w;
+        }
+      }
+    }
+    constexpr int ROWS = 64 / PIECES;  // of one store
+#pragma unroll
+    for (int s = 0; s < AT_ONCE * 16 / ROWS; ++s) {
+      if (j0 + s * ROWS / 16 >= A) continue;
+      const int row = s * ROWS + lane / PIECES, piece = lane % PIECES;
+      const i32x4 w = *reinterpret_cast<const i32x4*>(mine + row * WIDTH + ((piece ^ (row & (PIECES - 1) & 7)) << 4));
+      const int r = (Cfg::WR * (j0 + row / 16) + wr) * 16 + row % 16, c = wc0 + piece * VALUES;
+      if (r >= o.rows || c >= o.cols) continue;
+      Out* to = static_cast<Out*>(o.base) + (int64_t)r * o.ld + c;
+      if (c + VALUES <= o.cols) {
+        __builtin_memcpy(to, &w, 16);  // (memory takes 16 bytes anywhere)
+      } else {
+        Out v[VALUES];
+        __builtin_memcpy(v, &w, 16);
+#pragma unroll
+        for (int q = 0; q < VALUES; ++q)
+          if (c + q < o.cols) to[q] = v[q];
+      }
+    }
+  }
+}
+
+template <class Cfg, int A, class Acc, class Scale>
+__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[A][Cfg::TC], const Scale& scale, char* lds) {
+  barrier();  // every wavefront is done with the operands
+  if (o.type == kFloat32) store_tile_as<Cfg, float, A>(o, acc, scale, lds);
+  else if (o.type == kBFloat16) store_tile_as<Cfg, __bf16, A>(o, acc, scale, lds);
+  else store_tile_as<Cfg, _Float16, A>(o, acc, scale, lds);
+}
 
 // ---- kernels -------------------------------------------------------------------------------
 
@@ -606,7 +703,6 @@ struct RowProblem {
   void* y;
   int64_t ldy;         // elements
   int out_type;
-  int wide;
   const float* token_scale;    // 8-bit product only
   const float* channel_scale;
 };
@@ -633,11 +729,10 @@ __device__ __forceinline__ void row_tile(const RowProblem& p, const RowTile& til
   o.rows = tile.rows;
   o.cols = c.valid;
   o.type = p.out_type;
-  o.wide = p.wide;
   if constexpr (E::SIZE == 1)
-    store_tile<Cfg, A>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0});
+    store_tile<Cfg, A>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0}, lds);
   else
-    store_tile<Cfg, A>(o, acc, Unscaled{});
+    store_tile<Cfg, A>(o, acc, Unscaled{}, lds);
 }
 
 template <class E, Layout LC, Source S, class Cfg, int A>
@@ -747,7 +842,7 @@ __device__ __forceinline__ void few_rows_tile(const RowProblem& p, const RowTile
 #pragma unroll
     for (int q = 0; q < FewTile::WAVES; ++q) v += sums[(q * A * 16 + r) * STRIDE + c];
     float out;
-    if constexpr (E::SIZE == 1) out = TokenChannel{p.token_scale + tile.row, p.channel_scale + c0}(r, c, v);
+    if constexpr (E::SIZE == 1) out = (float)v * p.token_scale[tile.row + r] * p.channel_scale[c0 + c];
     else out = v;
     store_value(p.y, (int64_t)(tile.row + r) * p.ldy + c0 + c, p.out_type, out);
   }
@@ -776,59 +871,105 @@ struct SumProblem {
   void* d;
   int64_t ldd, stride_d;  // elements
   int out_type;
-  int wide;
+  int parts;              // > 1: each expert's rows are cut into that many parts, whose sums go to `partials`
+  float* partials;        // [parts][experts][rows][cols]
 };
 
-// Workgroup -> expert and tile of its matrix.  Experts differ in their rows, so each one's tiles are
-// spread over all XCDs, and each XCD has a contiguous part of them.
-__device__ __forceinline__ bool locate_sum(int wg, int experts, int tiles_r, int tiles_c, int& e, int& tr, int& tc) {
-  const int64_t tiles = (int64_t)tiles_r * tiles_c;
-  const int64_t chunk = (tiles + 7) >> 3;
-  const int64_t slot = wg >> 3;
-  e = (int)(slot / chunk);
-  const int64_t t = (wg & 7) * chunk + slot % chunk;
-  if (e >= experts || t >= tiles) return false;
-  constexpr int GR = 8;
-  const int64_t per = (int64_t)GR * tiles_c;
-  const int band = (int)(t / per), in_band = (int)(t - band * per);
-  const int rows = min(GR, tiles_r - band * GR);
-  tr = band * GR + in_band % rows;
-  tc = in_band / rows;
+struct SumTile {
+  int expert, part;
+  int begin, end;  // rows to sum over
+  int tile_r, tile_c;
+};
+
+// Workgroup -> expert, part and tile of its matrix.  Experts differ in their rows, so each one's tiles
+// are spread over all XCDs, and each XCD has a contiguous part of them.  Up to 64 experts are taken in
+// the order of their rows, the most first: the last workgroups to start are then short ones.
+__device__ __forceinline__ bool locate_sum(const SumProblem& p, unsigned wg, SumTile& tile) {
+  const unsigned tiles_r = p.tiles_r, tiles_c = p.tiles_c, tiles = tiles_r * tiles_c;
+  const unsigned chunk = (tiles + 7) >> 3;
+  const unsigned slot = wg >> 3, nth = slot / chunk;
+  const unsigned t = (wg & 7) * chunk + slot - nth * chunk;
+  const unsigned place = nth / (unsigned)p.parts;
+  tile.part = __builtin_amdgcn_readfirstlane((int)(nth - place * p.parts));
+  const int experts = p.groups.experts;
+  if (place >= (unsigned)experts || t >= tiles) return false;
+  constexpr unsigned GR = 8;
+  const unsigned per = GR * tiles_c;
+  const unsigned band = t / per, in_band = t - band * per;
+  const unsigned rows = min(GR, tiles_r - band * GR);
+  const unsigned column = in_band / rows;
+  tile.tile_r = __builtin_amdgcn_readfirstlane((int)(band * GR + in_band - column * rows));
+  tile.tile_c = __builtin_amdgcn_readfirstlane((int)column);
+  int begin, end, expert = (int)place;
+  if (experts > 1 && experts <= 64) {
+    const int lane = threadIdx.x & 63;
+    begin = end = 0;
+    if (lane < experts) group_rows(p.groups, lane, begin, end);
+    const int count = end - begin;
+    int before = 0;
+    for (int e = 0; e < experts; ++e) {
+      const int other = __builtin_amdgcn_readlane(count, e);
+      before += other > count || (other == count && e < lane);
+    }
+    expert = __ffsll((unsigned long long)__ballot(lane < experts && before == (int)place)) - 1;
+    expert = __builtin_amdgcn_readfirstlane(expert);
+    begin = __builtin_amdgcn_readlane(begin, expert);
+    end = __builtin_amdgcn_readlane(end, expert);
+  } else {
+    group_rows(p.groups, expert, begin, end);
+    begin = __builtin_amdgcn_readfirstlane(begin);
+    end = __builtin_amdgcn_readfirstlane(end);
+  }
+  tile.expert = __builtin_amdgcn_readfirstlane(expert);
+  if (p.parts > 1) {  // in units of 64 rows
+    const unsigned slabs = (unsigned)(end - begin + 63) >> 6, parts = p.parts, part = tile.part;
+    const unsigned each = slabs / parts, larger = slabs - each * parts;
+    const int first = (int)(part * each + min(part, larger)) << 6;
+    const int last = first + ((int)(each + (part < larger ? 1 : 0)) << 6);
+    end = min(end, begin + last);
+    begin = min(end, begin + first);
+  }
+  tile.begin = __builtin_amdgcn_readfirstlane(begin);
+  tile.end = __builtin_amdgcn_readfirstlane(end);
   return true;
+}
+
+// Where a tile's sums go: the expert's matrix, or this part's.
+__device__ __forceinline__ Result sum_result(const SumProblem& p, const SumTile& tile, int r0, int c0) {
+  Result o;
+  o.ld = p.parts > 1 ? p.cols : p.ldd;
+  o.type = p.parts > 1 ? (int)kFloat32 : p.out_type;
+  const int64_t at = (int64_t)r0 * o.ld + c0;
+  if (p.parts > 1) o.base = p.partials + ((int64_t)tile.part * p.groups.experts + tile.expert) * p.rows * p.cols + at;
+  else o.base = static_cast<char*>(p.d) + ((int64_t)tile.expert * p.stride_d + at) * type_bytes(p.out_type);
+  return o;
 }
 
 template <class E, Source SR, Source SC, class Cfg>
 __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
   using Product = TileProduct<E, XC, SR, XC, SC, Cfg>;
+  constexpr bool CODES = SC == Codes || SC == AnyCodes;
   __shared__ __attribute__((aligned(1024))) char lds[Product::LDS_BYTES];
-  int e, tr, tc;
-  if (!locate_sum(blockIdx.x, p.groups.experts, p.tiles_r, p.tiles_c, e, tr, tc)) return;
-  int begin, end;
-  group_rows(p.groups, e, begin, end);
-  begin = __builtin_amdgcn_readfirstlane(begin);
-  end = __builtin_amdgcn_readfirstlane(end);
-  const int r0 = tr * Cfg::BR, c0 = tc * Cfg::BC;
+  SumTile tile;
+  if (!locate_sum(p, blockIdx.x, tile)) return;
+  const int r0 = tile.tile_r * Cfg::BR, c0 = tile.tile_c * Cfg::BC;
   Operand r, c;
-  r.base = p.r + (int64_t)begin * p.ldr + (int64_t)r0 * E::SIZE;
+  r.base = p.r + (int64_t)tile.begin * p.ldr + (int64_t)r0 * E::SIZE;
   r.ld = p.ldr;
   r.valid = min(Cfg::BR, p.rows - r0);
-  c.base = p.c + (int64_t)begin * p.ldc + (int64_t)c0 * (SC == Codes ? 1 : E::SIZE);
+  c.base = p.c + (int64_t)tile.begin * p.ldc + (int64_t)c0 * (CODES ? 1 : E::SIZE);
   c.ld = p.ldc;
   c.valid = min(Cfg::BC, p.cols - c0);
   r.exponents = nullptr;
   r.ld_exp = 0;
-  c.exponents = SC == Codes ? p.exponents + (int64_t)begin * p.ld_exp + c0 / 128 : nullptr;
+  c.exponents = CODES ? p.exponents + (int64_t)tile.begin * p.ld_exp + c0 / 128 : nullptr;
   c.ld_exp = p.ld_exp;
   typename E::Acc acc[Cfg::TR][Cfg::TC];
-  Product::run(r, c, end - begin, lds, acc);
-  Result o;
-  o.base = static_cast<char*>(p.d) + ((int64_t)e * p.stride_d + (int64_t)r0 * p.ldd + c0) * type_bytes(p.out_type);
-  o.ld = p.ldd;
+  Product::run(r, c, tile.end - tile.begin, lds, acc);
+  Result o = sum_result(p, tile, r0, c0);
   o.rows = r.valid;
   o.cols = c.valid;
-  o.type = p.out_type;
-  o.wide = p.wide;
-  store_tile<Cfg, Cfg::TR>(o, acc, Unscaled{});
+  store_tile<Cfg, Cfg::TR>(o, acc, Unscaled{}, lds);
 }
 
 // ---- fp32 ----------------------------------------------------------------------------------
@@ -870,17 +1011,15 @@ __global__ __launch_bounds__(Cfg::NT) void row_product_f32_kernel(RowProblem p, 
 template <class Cfg>
 __global__ __launch_bounds__(Cfg::NT) void sum_product_f32_kernel(SumProblem p, int vec_dy, int vec_x) {
   __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
-  int e, tr, tc;
-  if (!locate_sum(blockIdx.x, p.groups.experts, p.tiles_r, p.tiles_c, e, tr, tc)) return;
-  int begin, end;
-  group_rows(p.groups, e, begin, end);
-  const int r0 = tr * Cfg::BN, c0 = tc * Cfg::BM;
+  SumTile tile;
+  if (!locate_sum(p, blockIdx.x, tile)) return;
+  const int r0 = tile.tile_r * Cfg::BN, c0 = tile.tile_c * Cfg::BM;
   const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
-  const float* dy = reinterpret_cast<const float*>(p.r) + (int64_t)begin * ldr + r0;
-  const float* x = reinterpret_cast<const float*>(p.c) + (int64_t)begin * ldc + c0;
-  float* d = static_cast<float*>(p.d) + (int64_t)e * p.stride_d + (int64_t)r0 * p.ldd + c0;
-  f32_tile<Cfg>(x, ldc, 0, dy, ldr, 1, min(Cfg::BM, p.cols - c0), min(Cfg::BN, p.rows - r0), end - begin, d, p.ldd,
-                vec_x, vec_dy, smem);
+  const float* dy = reinterpret_cast<const float*>(p.r) + (int64_t)tile.begin * ldr + r0;
+  const float* x = reinterpret_cast<const float*>(p.c) + (int64_t)tile.begin * ldc + c0;
+  const Result o = sum_result(p, tile, r0, c0);
+  f32_tile<Cfg>(x, ldc, 0, dy, ldr, 1, min(Cfg::BM, p.cols - c0), min(Cfg::BN, p.rows - r0), tile.end - tile.begin,
+                static_cast<float*>(o.base), o.ld, vec_x, vec_dy, smem);
 }
 
 // ---- 8-bit codes ---------------------------------------------------------------------------

@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from .ops._common import native_call, require_device_tensor
+from .ops._common import native_call, native_library, require_device_tensor, scratch
 
 __all__ = [
     "ActivationCheckpoint",
@@ -264,8 +264,10 @@ def expert_weight_gradient(
         values, saved = restore_activations(x), False  # the matrix cores take no 8-bit values beside fp32
     gradient, ldg = _rows(gradient)
     values, ldx = _rows(values)
+    nbytes = native_library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, outputs, inputs)
+    work = scratch(nbytes, gradient.device) if nbytes else None
     tail = (pointer, experts, tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out),
-            out.stride(0) if experts > 1 else 0)
+            out.stride(0) if experts > 1 else 0, work.data_ptr() if nbytes else 0, nbytes)
     if saved:
         _launch(index, "soapmi_expert_weight_gradient_saved", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx,
                 exponents.data_ptr(), _row_stride(exponents), *tail)

@@ -7,7 +7,7 @@ terms of fp32); the result is rounded once to its type, by half a step of the va
 import pytest
 import torch
 
-from soap_tp_amd import products
+from soap_tp_amd import _native, products
 
 pytestmark = pytest.mark.gpu
 
@@ -79,6 +79,8 @@ SHAPES = [
     (1, 1, 8, 8), (1, 3, 16, 64), (2, 2, 1, 1), (16, 4, 32, 128), (17, 2, 33, 65), (33, 70, 40, 24), (100, 130, 24, 136),
     (127, 1, 128, 64), (128, 1, 127, 63), (129, 2, 136, 200), (300, 5, 72, 72), (257, 3, 130, 1), (64, 2, 1, 130),
     (500, 2, 264, 328), (1000, 4, 257, 129), (700, 1, 512, 1040),
+    # long sums for few results: cut into parts
+    (4100, 1, 136, 72), (5000, 2, 130, 257), (1100, 1, 8, 8),
 ]
 
 
@@ -86,6 +88,30 @@ SHAPES = [
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 def test_layer_products(device, shape, dtype):
     check_layer(device, dtype, *shape, seed=sum(shape))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_long_sums_with_and_without_a_workspace(device, dtype):
+    """Through the C entry point: whole sums without a workspace, parts with one, and one that is too small."""
+    tokens, outputs, inputs = 6000, 72, 80
+    x, dy = values(device, 1, tokens, inputs, dtype=dtype), values(device, 2, tokens, outputs, dtype=dtype)
+    need = _native.library().soapmi_expert_weight_gradient_workspace_bytes(1, tokens, outputs, inputs)
+    assert need >= 2 * outputs * inputs * 4
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    expected, magnitudes = sums_exact(dy, x, [(0, tokens)])[0], sums_exact(dy.abs(), x.abs(), [(0, tokens)])[0]
+
+    def call(workspace, nbytes):
+        dw = torch.empty(outputs, inputs, device=device)
+        _native.call("soapmi_expert_weight_gradient", code, dy.data_ptr(), outputs, x.data_ptr(), inputs, None, 1, tokens,
+                     outputs, inputs, 0, dw.data_ptr(), inputs, 0, workspace, nbytes,
+                     torch.cuda.current_stream(device).cuda_stream)
+        return dw
+
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    assert_product(call(None, 0), expected, magnitudes, tokens)
+    assert_product(call(work.data_ptr(), need), expected, magnitudes, tokens)
+    with pytest.raises(ValueError, match="workspace holds"):
+        call(work.data_ptr(), need - 1)
 
 
 @pytest.mark.parametrize("dtype", HALF, ids=str)
@@ -98,18 +124,19 @@ def test_layer_products_on_the_widest_tiles(device, dtype, outputs, inputs):
 def test_rows_behind_the_last_expert(device, dtype):
     """New results have zeros there, a caller's buffer keeps what it had; NaN in such rows reaches nothing."""
     x, weights, dy, spans, ends = check_layer(device, dtype, 200, 3, 48, 56, seed=9, spare=37)
+    calm = {48: products.expert_product(x, weights, ends), 56: products.expert_input_gradient(dy, weights, ends)}
+    sums = products.expert_weight_gradient(dy, x, ends)
     x, dy = x.clone(), dy.clone()
     x[163:] = float("nan")
     dy[163:] = float("inf")
     for call, rows, width in ((products.expert_product, x, 48), (products.expert_input_gradient, dy, 56)):
-        clean = call(rows[:163], weights, ends)
+        clean = calm[width][:163]
         fresh = call(rows, weights, ends)
         assert torch.equal(fresh[:163], clean) and not fresh[163:].any()
         out = torch.full((200, width), 7.0, dtype=dtype, device=device)
         assert call(rows, weights, ends, out=out) is out
         assert torch.equal(out[:163], clean) and (out[163:] == 7).all()
-    assert torch.equal(products.expert_weight_gradient(dy, x, ends),
-                       products.expert_weight_gradient(dy[:163], x[:163], ends))
+    assert torch.equal(products.expert_weight_gradient(dy, x, ends), sums)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -217,6 +244,11 @@ def test_ends_out_of_order_stay_inside_the_buffers(device):
         assert products.expert_weight_gradient(dy, products.checkpoint_activations(x), ends).isfinite().all()
 
 
+def check_part(actual, a, b):
+    """Rows ``a`` times the matrix ``b``: other sizes may add in another order."""
+    assert_product(actual, torch.mm(a.double(), b.double()), torch.mm(a.double().abs(), b.double().abs()), a.shape[1])
+
+
 def test_offsets_beyond_32_bits(device):
     """Expert matrices and rows that start more than 2^32 bytes into their buffers."""
     inputs, outputs, experts = 4096, 8192, 72
@@ -227,29 +259,34 @@ def test_offsets_beyond_32_bits(device):
     ends[-1] = 40
     y = products.expert_product(x, weights, ends)
     assert not y[:20].any()
-    assert torch.equal(y[20:], products.expert_product(x[20:], weights[-1], None))
+    check_part(y[20:], x[20:], weights[-1].t())
     dy = values(device, 3, 40, outputs, dtype=torch.bfloat16)
     dx = products.expert_input_gradient(dy, weights, ends)
-    assert not dx[:20].any() and torch.equal(dx[20:], products.expert_input_gradient(dy[20:], weights[-1], None))
+    assert not dx[:20].any()
+    check_part(dx[20:], dy[20:], weights[-1])
     products.expert_weight_gradient(dy, x, ends, out=weights)
-    assert torch.equal(weights[-1], products.expert_weight_gradient(dy[20:], x[20:], None, out_dtype=torch.bfloat16))
+    check_part(weights[-1], dy[20:].t(), x[20:])
+    assert not weights[1:-1].any()
     del weights
     rows = 2200000  # of 1024 values in 16 bits: 4.5e9 bytes
     tall = torch.zeros(rows, 1024, dtype=torch.bfloat16, device=device)
     tall[-100:] = values(device, 4, 100, 1024, dtype=torch.bfloat16)
     small = values(device, 5, 16, 1024, dtype=torch.bfloat16)
+    pair = torch.stack([small, small])
     ends = torch.tensor([rows - 100, rows], device=device)
-    y = products.expert_product(tall, torch.stack([small, small]), ends)
-    assert not y[:-100].any() and torch.equal(y[-100:], products.expert_product(tall[-100:], small, None))
-    grown = products.expert_input_gradient(y, torch.stack([small, small]), ends)
-    assert torch.equal(grown[-100:], products.expert_input_gradient(y[-100:], small, None)) and not grown[:-100].any()
+    y = products.expert_product(tall, pair, ends)
+    assert not y[:-100].any()
+    check_part(y[-100:], tall[-100:], small.t())
+    grown = products.expert_input_gradient(y, pair, ends)
+    assert not grown[:-100].any()
+    check_part(grown[-100:], y[-100:], small)
     dw = products.expert_weight_gradient(y, tall, ends)
-    assert not dw[0].any() and torch.equal(dw[1], products.expert_weight_gradient(y[-100:], tall[-100:], None))
+    assert not dw[0].any()
+    check_part(dw[1], y[-100:].t(), tall[-100:])
     saved = products.checkpoint_activations(tall)
-    assert torch.equal(products.expert_weight_gradient(y, saved, ends)[1],
-                       products.expert_weight_gradient(y[-100:], products.checkpoint_activations(tall[-100:]), None))
-    assert torch.equal(products.restore_activations(saved)[-100:],
-                       products.restore_activations(products.checkpoint_activations(tall[-100:])))
+    part = products.checkpoint_activations(tall[-100:])
+    check_part(products.expert_weight_gradient(y, saved, ends)[1], y[-100:].t(), products.restore_activations(part))
+    assert torch.equal(products.restore_activations(saved)[-100:], products.restore_activations(part))
 
 
 # ---- activation checkpoints ----------------------------------------------------------------
@@ -323,7 +360,7 @@ def test_checkpoint_and_restore(device, dtype, rows, columns):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("shape", [(1, 1, 8, 8), (17, 2, 33, 65), (33, 70, 40, 24), (129, 2, 136, 200), (300, 5, 72, 328),
-                                   (500, 2, 264, 520), (700, 1, 130, 1)], ids=str)
+                                   (500, 2, 264, 520), (700, 1, 130, 1), (4100, 1, 136, 72), (5000, 2, 130, 257)], ids=str)
 def test_weight_gradient_from_a_checkpoint(device, dtype, shape):
     tokens, experts, outputs, inputs = shape
     x = values(device, 1, tokens, inputs, dtype=dtype) * values(device, 2, 1, inputs, dtype=dtype)

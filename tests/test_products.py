@@ -131,11 +131,11 @@ def test_checkpoint_and_int8_refusals():
     ("soapmi_expert_product", (0, P, 4, P, 8, 32, 1, P, 2, 6, 4, 8, 0, P, 4, 0, None), "leading dimensions"),
     ("soapmi_expert_product", (0, P, 8, P, 8, -1, 0, P, 2, 6, 4, 8, 0, P, 4, 0, None), "stride_w must be"),
     ("soapmi_expert_product", (0, P, 8, None, 8, 32, 0, P, 2, 6, 4, 8, 0, P, 4, 0, None), "nonzero"),
-    ("soapmi_expert_weight_gradient", (0, P, 4, P, 8, P, 2, 6, 4, 8, 0, P, 8, 31, None), "must not overlap"),
-    ("soapmi_expert_weight_gradient", (0, P, 3, P, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None), "leading dimensions"),
-    ("soapmi_expert_weight_gradient", (0, P, 4, None, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None), "nonzero"),
-    ("soapmi_expert_weight_gradient_saved", (0, P, 4, P, 8, P, 1, P, 2, 6, 4, 8, 0, P, 8, 32, None), "restore a float32"),
-    ("soapmi_expert_weight_gradient_saved", (1, P, 4, P, 8, P, 0, P, 2, 6, 4, 8, 0, P, 8, 32, None), "leading dimensions"),
+    ("soapmi_expert_weight_gradient", (0, P, 4, P, 8, P, 2, 6, 4, 8, 0, P, 8, 31, None, 0, None), "must not overlap"),
+    ("soapmi_expert_weight_gradient", (0, P, 3, P, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "leading dimensions"),
+    ("soapmi_expert_weight_gradient", (0, P, 4, None, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "nonzero"),
+    ("soapmi_expert_weight_gradient_saved", (0, P, 4, P, 8, P, 1, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "restore a float32"),
+    ("soapmi_expert_weight_gradient_saved", (1, P, 4, P, 8, P, 0, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "leading dimensions"),
     ("soapmi_checkpoint_activations", (0, P, 8, 6, 8, P, 8, P, 0, None), "leading dimensions"),
     ("soapmi_checkpoint_activations", (0, None, 8, 6, 8, P, 8, P, 1, None), "nonzero"),
     ("soapmi_restore_activations", (7, P, 8, P, 1, 6, 8, P, 8, None), "dtype must be 0"),
@@ -151,7 +151,7 @@ def test_entry_points_refuse(name, arguments, message):
 @pytest.mark.parametrize("name,arguments", [
     ("soapmi_expert_product", (1, None, 8, None, 8, 32, 0, P, 0, 0, 4, 8, 1, None, 4, 1, None)),
     ("soapmi_expert_product", (1, None, 8, None, 8, 0, 0, None, 1, 6, 0, 8, 1, None, 0, 1, None)),
-    ("soapmi_expert_weight_gradient", (1, None, 4, None, 0, None, 1, 6, 4, 0, 1, None, 0, 0, None)),
+    ("soapmi_expert_weight_gradient", (1, None, 4, None, 0, None, 1, 6, 4, 0, 1, None, 0, 0, None, 0, None)),
     ("soapmi_checkpoint_activations", (1, None, 8, 0, 8, None, 8, None, 1, None)),
     ("soapmi_restore_activations", (1, None, 0, None, 0, 0, 0, None, 0, None)),
     ("soapmi_quantize_rows", (1, None, 8, 0, 8, None, 8, None, None)),
