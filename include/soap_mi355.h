@@ -225,20 +225,13 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
                                   size_t workspace_bytes, void* stream);
 size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t tokens, int64_t n, int64_t k);
 
-/* The same with x as soapmi_checkpoint_activations saved it from values of `dtype` (16-bit types only: a
- * fp32 checkpoint is restored first).  The codes' steps are powers of two, so x enters the product
- * exactly as it is restored.  Where ldq is a multiple of 8, codes behind a row's last one, up to the next
- * multiple of 8, may be read (every row, the last one too, has ldq of them). */
-int soapmi_expert_weight_gradient_saved(int dtype, const void* gradient, int64_t ldg, const int8_t* codes, int64_t ldq,
-                                        const uint8_t* exponents, int64_t lde, const int64_t* ends, int64_t experts,
-                                        int64_t tokens, int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw,
-                                        int64_t stride_dw, void* workspace, size_t workspace_bytes, void* stream);
-
 /* Activation checkpoint of a rows x cols matrix: 8-bit codes (rows x cols) and an exponent for each row
  * and 128 columns (rows x ceil(cols / 128)).  With 2^(p-1) <= m < 2^p the largest magnitude of those
  * columns, step = 2^max(p-7, -126) (fp16: 2^max(p-7, -24)), code = round-to-even(x / step) held to
  * -127..127, exponent = log2(step) + 127.  A value is restored as code * step, off by at most half a step
- * (one step above 127.5 steps).  Columns that hold an infinity or NaN get exponent 255 and are restored as NaN. */
+ * (one step above 127.5 steps).  Columns that hold an infinity or NaN get exponent 255 and are restored as NaN.
+ * A step is a power of two, so that code * step is exact in the type it came from: a weight gradient's
+ * products of restored values are those of the codes. */
 int soapmi_checkpoint_activations(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes,
                                   int64_t ldq, uint8_t* exponents, int64_t lde, void* stream);
 int soapmi_restore_activations(int dtype, const int8_t* codes, int64_t ldq, const uint8_t* exponents, int64_t lde,

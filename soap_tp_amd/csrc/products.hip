@@ -11,8 +11,8 @@ extern template int row_products<ElemBF16, XC>(hipStream_t, const RowProblem&, b
 extern template int row_products<ElemF16, KC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemF16, XC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemI8, KC>(hipStream_t, const RowProblem&, bool);
-extern template int sum_products<ElemBF16>(hipStream_t, const SumProblem&, bool, bool);
-extern template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool, bool);
+extern template int sum_products<ElemBF16>(hipStream_t, const SumProblem&, bool);
+extern template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool);
 
 // The parts' sums, added in order.
 static __global__ __launch_bounds__(256) void join_parts_kernel(SumProblem p) {
@@ -128,7 +128,8 @@ template <class T>
 int launch_quantize(hipStream_t stream, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldq,
                     float* scales) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
+                      ldq * 64 < kBufferBytes;
   // Long rows, and few rows, take a workgroup each; short ones a wavefront.
   if (cols > 1024)
     hipLaunchKernelGGL((quantize_rows_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, stream, x, ldx, (int)rows,
@@ -144,7 +145,8 @@ template <class T>
 int launch_checkpoint(hipStream_t stream, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldq,
                       uint8_t* exponents, int64_t lde, int lowest) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
+                      ldq * 64 < kBufferBytes;
   const int64_t blocks = ceil_div64(cols, kCheckpointBlock);
   const int64_t grid = ceil_div64(rows * blocks, 16);
   SOAPMI_REQUIRE(grid < (int64_t)1 << 31, "the matrix has too many blocks for one launch");
@@ -158,7 +160,8 @@ template <class T>
 int launch_restore(hipStream_t stream, const int8_t* codes, int64_t ldq, const uint8_t* exponents, int64_t lde, int64_t rows,
                    int64_t cols, T* x, int64_t ldx) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
+                      ldq * 64 < kBufferBytes;
   const int64_t pieces = ceil_div64(cols, 8);
   const int64_t grid = ceil_div64(rows * pieces, 256);
   SOAPMI_REQUIRE(grid < (int64_t)1 << 31, "the matrix is too large for one launch");
@@ -243,29 +246,7 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
     return launch_sums_f32<F32Tile>(s, p, vec_dy, vec_x);
   }
   const bool direct = direct_ok(gradient, p.ldr, n * 2, 64) && direct_ok(x, p.ldc, k * 2, 64);
-  return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct, false) : sum_products<ElemF16>(s, p, direct, false);
-}
-
-int soapmi_expert_weight_gradient_saved(int dtype, const void* gradient, int64_t ldg, const int8_t* codes, int64_t ldq,
-                                        const uint8_t* exponents, int64_t lde, const int64_t* ends, int64_t experts,
-                                        int64_t tokens, int64_t n, int64_t k, int out_dtype, void* dw, int64_t lddw,
-                                        int64_t stride_dw, void* workspace, size_t workspace_bytes, void* stream) {
-  if (int rc = check_gradient(dtype, out_dtype, ends, experts, tokens, n, k, ldg, ldq, lddw, stride_dw)) return rc;
-  SOAPMI_REQUIRE(dtype != kFloat32, "dtype must be 1 (bfloat16) or 2 (float16): restore a float32 checkpoint first");
-  SOAPMI_REQUIRE(lde >= ceil_div64(k, kCheckpointBlock), "leading dimensions are too small");
-  if (experts == 0 || n == 0 || k == 0) return kOk;
-  SOAPMI_REQUIRE(dw && (tokens == 0 || (gradient && codes && exponents)), "buffer addresses must be nonzero");
-  SumProblem p;
-  if (int rc = sum_problem(dtype, gradient, ldg, ends, experts, tokens, n, k, out_dtype, dw, lddw, stride_dw, workspace,
-                           workspace_bytes, &p))
-    return rc;
-  p.c = reinterpret_cast<const char*>(codes);
-  p.ldc = ldq;
-  p.exponents = exponents;
-  p.ld_exp = lde;
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool direct = direct_ok(gradient, p.ldr, n * 2, 64) && reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
-  return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct, true) : sum_products<ElemF16>(s, p, direct, true);
+  return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct) : sum_products<ElemF16>(s, p, direct);
 }
 
 size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t tokens, int64_t n, int64_t k) {

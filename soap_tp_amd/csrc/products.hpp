@@ -186,18 +186,13 @@ __device__ __forceinline__ int column_of(int i, int m) { return 32 * (i >> 1) + 
 
 enum Layout { KC, XC };
 // How an operand gets to LDS.  Direct: 16-byte pieces straight from memory (aligned operands).  Staged:
-// through registers, any alignment and size.  Codes: through registers, 8-bit codes of an activation
-// checkpoint expanded to 16-bit values on the way, rows of whole, aligned pieces.  AnyCodes: codes of any
-// alignment and size.
-enum Source { Direct, Staged, Codes, AnyCodes };
+// through registers, any alignment and size.
+enum Source { Direct, Staged };
 
 struct Operand {
   const char* base;  // tile's first element
   int64_t ld;        // bytes from one stored row to the next
   int valid;         // rows (columns) of the tile that exist
-  // Codes only: exponents[k * ld_exp], of the tile's first row and first block
-  const uint8_t* exponents;
-  int64_t ld_exp;
 };
 
 constexpr unsigned kOutside = 0xC0000000u;    // a byte offset outside every buffer: such a lane fetches zeros
@@ -256,8 +251,6 @@ struct Loader {
   static constexpr int PIECES = BYTES / 16;
   static constexpr int NP = (PIECES + NT - 1) / NT;
   static_assert(L == KC || E::SIZE == 2, "transposing reads are of 16-bit values");
-  static constexpr bool CODES = S == Codes || S == AnyCodes;
-  static_assert(!CODES || L == XC, "codes are expanded along x");
   static_assert(S != Direct || PIECES % 64 == 0, "whole wavefronts fetch");
   static constexpr int PER_ROW = L == KC ? 8 : BX * E::SIZE / 16;  // pieces in an LDS row
 
@@ -269,15 +262,11 @@ struct Loader {
   const char* base;
   int64_t ld;
   int valid;
-  const uint8_t* exponents;
-  int64_t ld_exp;
   int tid;
   unsigned offset, offset_now;  // Direct: of the lane's first piece; in the slab being sent
   int first_row, first_piece;   // of the lane's first piece
   i32x4 resource;
-  struct Two { unsigned w[2]; };
-  std::conditional_t<CODES, Two, i32x4> held[S == Direct ? 1 : AHEAD][S == Direct ? 1 : NP];  // slabs in registers
-  int held_exp[CODES ? AHEAD : 1][CODES ? NP : 1];
+  i32x4 held[S == Direct ? 1 : AHEAD][S == Direct ? 1 : NP];  // Staged: slabs in registers
 
   // stored row and piece of LDS piece q
   static __device__ __forceinline__ void place(int q, int& row, int& piece) {
@@ -291,8 +280,6 @@ struct Loader {
     base = o.base;
     ld = o.ld;
     valid = o.valid;
-    exponents = o.exponents;
-    ld_exp = o.ld_exp;
     tid = tid_;
     place(tid, first_row, first_piece);
     if constexpr (S == Direct) {
@@ -319,47 +306,21 @@ struct Loader {
     load_to_lds(resource, offset_now, (unsigned)(i * STEP * (int)ld), lds + wave * 1024 + i * NT * 16);
   }
 
-  // Other sources: piece i of slab kt comes to register set `set`.  k_left as for aim().
+  // Staged: piece i of slab kt comes to register set `set`.  k_left as for aim().
   __device__ __forceinline__ void fetch(int i, int kt, int k_left, int set) {
-    if constexpr (S != Direct) {
+    if constexpr (S == Staged) {
       if (PIECES % NT != 0 && tid + i * NT >= PIECES) return;
       const int row = first_row + i * STEP;
-      if constexpr (S == Staged) {
-        const char* at = slab(kt) + first_piece * 16;
-        if (L == KC) {
-          const int r = min(row, valid - 1);  // rows behind the last one only reach results that are not stored
-          at += r * ld;
-          if (k_left >= SLAB_K) held[set][i] = load_bytes(at, 16);
-          else held[set][i] = load_bytes(at, k_left * E::SIZE - first_piece * 16);
-        } else {
-          at += row * ld;
-          if (k_left >= SLAB_K && valid == BX) held[set][i] = load_bytes(at, 16);
-          else held[set][i] = load_bytes(at, row < k_left ? valid * E::SIZE - first_piece * 16 : 0);
-        }
-      } else if constexpr (S == Codes) {
-        // eight codes for a piece of eight 16-bit values; a row behind the last one is the slab's first with
-        // step zero, a slab behind the last one the first slab, and columns behind the last one are whatever
-        // stands there: they only reach results that are not stored
-        const bool inside = row < k_left;
-        const int kt_inside = k_left > 0 ? kt : 0;
-        const char* at = slab(kt_inside) + (first_piece * 8 < valid ? first_piece * 8 : 0);
-        const uint8_t* steps = exponents + (int64_t)kt_inside * 64 * ld_exp + (first_piece * 8 < valid ? first_piece >> 4 : 0);
-        const int r = inside ? row : 0;
-        const unsigned e = steps[r * ld_exp];
-        __builtin_memcpy(&held[set][i], __builtin_assume_aligned(at + r * ld, 8), 8);
-        held_exp[set][i] = inside ? e : 0;
+      const char* at = slab(kt) + first_piece * 16;
+      if (L == KC) {
+        const int r = min(row, valid - 1);  // rows behind the last one only reach results that are not stored
+        at += r * ld;
+        if (k_left >= SLAB_K) held[set][i] = load_bytes(at, 16);
+        else held[set][i] = load_bytes(at, k_left * E::SIZE - first_piece * 16);
       } else {
-        const int count = row < k_left ? valid - first_piece * 8 : 0;
-        held[set][i] = Two{};
-        held_exp[set][i] = 0;
-        if (count > 0) {
-          const char* p = slab(kt) + row * ld + first_piece * 8;
-          held_exp[set][i] = exponents[((int64_t)kt * 64 + row) * ld_exp + (first_piece >> 4)];
-          char b[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) b[j] = j < count ? p[j] : 0;
-          __builtin_memcpy(&held[set][i], b, 8);
-        }
+        at += row * ld;
+        if (k_left >= SLAB_K && valid == BX) held[set][i] = load_bytes(at, 16);
+        else held[set][i] = load_bytes(at, row < k_left ? valid * E::SIZE - first_piece * 16 : 0);
       }
     }
   }
@@ -367,22 +328,8 @@ struct Loader {
   // ... and goes on to LDS.
   __device__ __forceinline__ void put(int i, int set, char* lds) {
     const int q = tid + i * NT;
-    if constexpr (S != Direct) {
-      if (PIECES % NT == 0 || q < PIECES) {
-        if constexpr (S == Staged) {
-          *reinterpret_cast<i32x4*>(lds + q * 16) = held[set][i];
-        } else {
-          // code * 2^e is exact in bf16 (8 bits of mantissa) and, with the exponents that
-          // checkpoints of fp16 values have, in fp16
-          const float step = exponent_value(held_exp[set][i]);
-          typename E::Scalar v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[j] = (typename E::Scalar)((float)(int8_t)(held[set][i].w[j >> 2] >> (8 * (j & 3))) * step);
-          __builtin_memcpy(lds + q * 16, v, 16);
-        }
-      }
-    }
+    if constexpr (S == Staged)
+      if (PIECES % NT == 0 || q < PIECES) *reinterpret_cast<i32x4*>(lds + q * 16) = held[set][i];
   }
 
   // 16 bytes of fragment data for (x, k step ks): KC: k pieces 4 ks + lane group; XC: 8 k values.
@@ -411,8 +358,8 @@ struct Loader {
   }
 };
 
-// BR x BC results, WR x WC wavefronts.  STAGES slabs are in LDS or on their way there (Direct operands;
-// with others two, and AHEAD more in registers).
+// BR x BC results, WR x WC wavefronts.  STAGES slabs are in LDS or on their way there (Direct; Staged: two,
+// and AHEAD more in registers).
 template <int BR_, int BC_, int WR_, int WC_, int STAGES_, int AHEAD_>
 struct ProductTile {
   static constexpr int BR = BR_, BC = BC_, WR = WR_, WC = WC_, STAGES = STAGES_, AHEAD = AHEAD_;
@@ -430,13 +377,13 @@ struct ProductTile {
 // the next step's come from LDS into other registers, and further slabs are in LDS or on their way.  What
 // moves data is dealt out between the rows of matrix instructions: a wavefront issues in order, and the
 // loads of a whole slab in a row would keep it from issuing anything else for as long as they take.
-template <class E, Layout LR, Source SR, Layout LC, Source SC, class Cfg, int A = Cfg::TR>
+template <class E, Layout LR, Layout LC, Source S, class Cfg, int A = Cfg::TR>
 struct TileProduct {
-  static constexpr bool DIRECT = SR == Direct && SC == Direct;
+  static constexpr bool DIRECT = S == Direct;
   static constexpr int STAGES = DIRECT ? Cfg::STAGES : 2, AHEAD = DIRECT ? 1 : Cfg::AHEAD;
   static_assert((STAGES & (STAGES - 1)) == 0, "a slab's stage is its number's low bits");
-  using LoadR = Loader<E, LR, SR, Cfg::BR, Cfg::NT, false, AHEAD>;
-  using LoadC = Loader<E, LC, SC, Cfg::BC, Cfg::NT, true, AHEAD>;
+  using LoadR = Loader<E, LR, S, Cfg::BR, Cfg::NT, false, AHEAD>;
+  using LoadC = Loader<E, LC, S, Cfg::BC, Cfg::NT, true, AHEAD>;
   static constexpr int SLAB_K = LoadR::SLAB_K;
   static_assert(LoadR::SLAB_K == LoadC::SLAB_K, "one slab for both operands");
   static_assert(!DIRECT || STAGES == 2 || (LoadR::PIECES % Cfg::NT == 0 && LoadC::PIECES % Cfg::NT == 0),
@@ -479,10 +426,12 @@ struct TileProduct {
     lc.init(c, tid);
     auto stage_of = [](int kt) { return (kt & (STAGES - 1)) * STAGE; };
     auto aim = [&](int kt) {
-      if constexpr (SR == Direct) lr.aim(kt, k_count - kt * SLAB_K);
-      if constexpr (SC == Direct) lc.aim(kt, k_count - kt * SLAB_K);
+      if constexpr (DIRECT) {
+        lr.aim(kt, k_count - kt * SLAB_K);
+        lc.aim(kt, k_count - kt * SLAB_K);
+      }
     };
-    // piece n of slab kt: to registers (operands that are not Direct) ...
+    // piece n of slab kt: to registers (Staged) ...
     auto fetch = [&](int n, int kt, int set) {
       if (n < PIECES_R) lr.fetch(n, kt, k_count - kt * SLAB_K, set);
       else lc.fetch(n - PIECES_R, kt, k_count - kt * SLAB_K, set);
@@ -490,26 +439,32 @@ struct TileProduct {
     // ... and to LDS, from there or straight from memory
     auto move = [&](int n, int kt, int set) {
       if (n < PIECES_R) {
-        if constexpr (SR == Direct) lr.send(n, lds_address + stage_of(kt));
+        if constexpr (DIRECT) lr.send(n, lds_address + stage_of(kt));
         else lr.put(n, set, lds + stage_of(kt));
       } else {
-        if constexpr (SC == Direct) lc.send(n - PIECES_R, lds_address + stage_of(kt) + LoadR::BYTES);
+        if constexpr (DIRECT) lc.send(n - PIECES_R, lds_address + stage_of(kt) + LoadR::BYTES);
         else lc.put(n - PIECES_R, set, lds + stage_of(kt) + LoadR::BYTES);
       }
     };
+    if constexpr (!DIRECT) {
+      static_assert(AHEAD >= STAGES, "the first slabs travel together");
+#pragma unroll
+      for (int kt = 0; kt < STAGES; ++kt)
+#pragma unroll
+        for (int n = 0; n < PIECES; ++n) fetch(n, kt, kt);
+    }
 #pragma unroll
     for (int kt = 0; kt < STAGES; ++kt) {
       aim(kt);
 #pragma unroll
-      for (int n = 0; n < PIECES; ++n) {
-        fetch(n, kt, 0);
-        move(n, kt, 0);
-      }
+      for (int n = 0; n < PIECES; ++n) move(n, kt, kt % AHEAD);
     }
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int set = 0; set < AHEAD; ++set)
+      for (int set = 0; set < AHEAD; ++set)
 #pragma unroll
-      for (int n = 0; n < PIECES; ++n) fetch(n, STAGES + set, set);
+        for (int n = 0; n < PIECES; ++n) fetch(n, STAGES + set, set);
+    }
     arrive<(STAGES - 1) * PIECES>();
     Fragments f0, f1;
 #pragma unroll
@@ -563,14 +518,8 @@ struct TileProduct {
   template <int LATER>
   static __device__ __forceinline__ void arrive() {
     if constexpr (DIRECT) wait_loads<LATER>();
-    else wait_loads_to_lds();
     wait_lds();
     barrier();
-  }
-  // With operands that pass through registers, the loads to LDS are not the only ones and cannot be
-  // counted from here: all are waited for (none, if no operand is Direct: LDS writes are waited for as such).
-  static __device__ __forceinline__ void wait_loads_to_lds() {
-    if constexpr (SR == Direct || SC == Direct) wait_loads<0>();
   }
 };
 
@@ -719,10 +668,8 @@ __device__ __forceinline__ void row_tile(const RowProblem& p, const RowTile& til
   c.base = p.c + (int64_t)tile.expert * p.stride_c + (LC == KC ? (int64_t)c0 * p.ldc : (int64_t)c0 * E::SIZE);
   c.ld = p.ldc;
   c.valid = min(Cfg::BC, p.cols - c0);
-  r.exponents = c.exponents = nullptr;
-  r.ld_exp = c.ld_exp = 0;
   typename E::Acc acc[A][Cfg::TC];
-  TileProduct<E, KC, S, LC, S, Cfg, A>::run(r, c, tile.expert >= p.groups.experts ? 0 : p.k, lds, acc);
+  TileProduct<E, KC, LC, S, Cfg, A>::run(r, c, tile.expert >= p.groups.experts ? 0 : p.k, lds, acc);
   Result o;
   o.base = static_cast<char*>(p.y) + ((int64_t)tile.row * p.ldy + c0) * type_bytes(p.out_type);
   o.ld = p.ldy;
@@ -745,7 +692,7 @@ __device__ __forceinline__ void row_tile_at_least(const RowProblem& p, const Row
 
 template <class E, Layout LC, Source S, class Cfg>
 __global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
-  __shared__ __attribute__((aligned(1024))) char lds[TileProduct<E, KC, S, LC, S, Cfg>::LDS_BYTES];
+  __shared__ __attribute__((aligned(1024))) char lds[TileProduct<E, KC, LC, S, Cfg>::LDS_BYTES];
   constexpr int GRAIN = 16 * Cfg::WR;
   RowTile tile;
   int tile_c;
@@ -862,10 +809,8 @@ __global__ __launch_bounds__(FewTile::NT) void few_rows_kernel(RowProblem p) {
 struct SumProblem {
   RowGroups groups;
   const char* r;          // tokens x rows
-  const char* c;          // tokens x cols (values, or codes)
+  const char* c;          // tokens x cols
   int64_t ldr, ldc;       // bytes
-  const uint8_t* exponents;
-  int64_t ld_exp;
   int rows, cols;
   int tiles_r, tiles_c;
   void* d;
@@ -945,10 +890,9 @@ __device__ __forceinline__ Result sum_result(const SumProblem& p, const SumTile&
   return o;
 }
 
-template <class E, Source SR, Source SC, class Cfg>
+template <class E, Source S, class Cfg>
 __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
-  using Product = TileProduct<E, XC, SR, XC, SC, Cfg>;
-  constexpr bool CODES = SC == Codes || SC == AnyCodes;
+  using Product = TileProduct<E, XC, XC, S, Cfg>;
   __shared__ __attribute__((aligned(1024))) char lds[Product::LDS_BYTES];
   SumTile tile;
   if (!locate_sum(p, blockIdx.x, tile)) return;
@@ -957,13 +901,9 @@ __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
   r.base = p.r + (int64_t)tile.begin * p.ldr + (int64_t)r0 * E::SIZE;
   r.ld = p.ldr;
   r.valid = min(Cfg::BR, p.rows - r0);
-  c.base = p.c + (int64_t)tile.begin * p.ldc + (int64_t)c0 * (CODES ? 1 : E::SIZE);
+  c.base = p.c + (int64_t)tile.begin * p.ldc + (int64_t)c0 * E::SIZE;
   c.ld = p.ldc;
   c.valid = min(Cfg::BC, p.cols - c0);
-  r.exponents = nullptr;
-  r.ld_exp = 0;
-  c.exponents = CODES ? p.exponents + (int64_t)tile.begin * p.ld_exp + c0 / 128 : nullptr;
-  c.ld_exp = p.ld_exp;
   typename E::Acc acc[Cfg::TR][Cfg::TC];
   Product::run(r, c, tile.end - tile.begin, lds, acc);
   Result o = sum_result(p, tile, r0, c0);
@@ -1139,7 +1079,8 @@ constexpr int kCheckpointBlock = 128;  // columns that share an exponent
 // step is 2^(p-7) (at least 2^-126; 2^-24, the smallest fp16 value, for fp16) and the codes are
 // round(x / step) held to -127..127; the exponent is stored with 127 added, 255 marks a block that holds
 // an infinity or NaN.  The step is a power of two because it stands inside the weight gradient's sum:
-// code * step and its product with a 16-bit gradient are then exact.  Sixteen lanes take a block.
+// code * step is then exact in 16 bits, and so is
+// its product with a 16-bit gradient in fp32.  Sixteen lanes take a block.
 template <class T>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, int blocks,
                                                          int vec_x, int8_t* codes, int64_t ldq, int vec_q,

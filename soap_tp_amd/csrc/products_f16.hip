@@ -4,5 +4,5 @@
 namespace soapmi {
 template int row_products<ElemF16, KC>(hipStream_t, const RowProblem&, bool);
 template int row_products<ElemF16, XC>(hipStream_t, const RowProblem&, bool);
-template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool, bool);
+template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool);
 }  // namespace soapmi

@@ -106,30 +106,28 @@ inline int sum_grid(SumProblem& p, int br, int bc, unsigned* grid) {
   return grid_of(8 * ceil_div64((int64_t)p.tiles_r * p.tiles_c, 8) * p.groups.experts * p.parts, grid);
 }
 
-template <class E, Source SR, Source SC, class Cfg>
+template <class E, Source S, class Cfg>
 int launch_sums(hipStream_t stream, SumProblem p) {
   unsigned grid;
   if (int rc = sum_grid(p, Cfg::BR, Cfg::BC, &grid)) return rc;
-  hipLaunchKernelGGL((sum_product_kernel<E, SR, SC, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
+  hipLaunchKernelGGL((sum_product_kernel<E, S, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return p.parts > 1 ? launch_join(stream, p) : kOk;
 }
 
 // Wide tiles from 192 of them on: SUMS_MEASURED
-template <class E, Source SR, Source SC>
+template <class E, Source S>
 int launch_sums(hipStream_t stream, const SumProblem& p) {
   const int64_t wide_tiles = ceil_div64(p.rows, 256) * ceil_div64(p.cols, 256) * p.groups.experts;
-  if constexpr (SR == Direct)
-    if (wide_tiles >= 96 && p.parts == 1) return launch_sums<E, SR, SC, WideTile>(stream, p);
-  return launch_sums<E, SR, SC, MidTile>(stream, p);
+  if constexpr (S == Direct)
+    if (wide_tiles >= 96 && p.parts == 1) return launch_sums<E, S, WideTile>(stream, p);
+  return launch_sums<E, S, MidTile>(stream, p);
 }
 
-// D_e = sums over the experts' rows.  direct: the operands may be fetched straight to LDS (saved: the
-// gradient may, and the codes' rows are whole aligned pieces).
+// D_e = sums over the experts' rows.  direct: the operands may be fetched straight to LDS.
 template <class E>
-int sum_products(hipStream_t stream, const SumProblem& p, bool direct, bool saved) {
-  if (saved) return direct ? launch_sums<E, Direct, Codes>(stream, p) : launch_sums<E, Staged, AnyCodes>(stream, p);
-  return direct ? launch_sums<E, Direct, Direct>(stream, p) : launch_sums<E, Staged, Staged>(stream, p);
+int sum_products(hipStream_t stream, const SumProblem& p, bool direct) {
+  return direct ? launch_sums<E, Direct>(stream, p) : launch_sums<E, Staged>(stream, p);
 }
 
 }  // namespace soapmi

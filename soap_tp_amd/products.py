@@ -260,19 +260,17 @@ def expert_weight_gradient(
         out = torch.empty(shape, dtype=out_dtype, device=gradient.device)
     if out.numel() == 0:
         return out
-    if saved and code == 0:
-        values, saved = restore_activations(x), False  # the matrix cores take no 8-bit values beside fp32
+    if saved:
+        # (restored for this product alone: expanding the codes inside the product kernel, tile by tile, was
+        # slower than reading the matrix once more)
+        values = restore_activations(x)
     gradient, ldg = _rows(gradient)
     values, ldx = _rows(values)
     nbytes = native_library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, outputs, inputs)
     work = scratch(nbytes, gradient.device) if nbytes else None
-    tail = (pointer, experts, tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out),
-            out.stride(0) if experts > 1 else 0, work.data_ptr() if nbytes else 0, nbytes)
-    if saved:
-        _launch(index, "soapmi_expert_weight_gradient_saved", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx,
-                exponents.data_ptr(), _row_stride(exponents), *tail)
-    else:
-        _launch(index, "soapmi_expert_weight_gradient", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx, *tail)
+    _launch(index, "soapmi_expert_weight_gradient", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx, pointer, experts,
+            tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out), out.stride(0) if experts > 1 else 0,
+            work.data_ptr() if nbytes else 0, nbytes)
     return out
 
 

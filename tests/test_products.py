@@ -134,8 +134,6 @@ def test_checkpoint_and_int8_refusals():
     ("soapmi_expert_weight_gradient", (0, P, 4, P, 8, P, 2, 6, 4, 8, 0, P, 8, 31, None, 0, None), "must not overlap"),
     ("soapmi_expert_weight_gradient", (0, P, 3, P, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "leading dimensions"),
     ("soapmi_expert_weight_gradient", (0, P, 4, None, 8, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "nonzero"),
-    ("soapmi_expert_weight_gradient_saved", (0, P, 4, P, 8, P, 1, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "restore a float32"),
-    ("soapmi_expert_weight_gradient_saved", (1, P, 4, P, 8, P, 0, P, 2, 6, 4, 8, 0, P, 8, 32, None, 0, None), "leading dimensions"),
     ("soapmi_checkpoint_activations", (0, P, 8, 6, 8, P, 8, P, 0, None), "leading dimensions"),
     ("soapmi_checkpoint_activations", (0, None, 8, 6, 8, P, 8, P, 1, None), "nonzero"),
     ("soapmi_restore_activations", (7, P, 8, P, 1, 6, 8, P, 8, None), "dtype must be 0"),
