@@ -21,7 +21,7 @@ INCLUDE_DIR = PACKAGE_DIR.parent / "include"
 # hardware-counter runs, where the profiled program should be a plain executable).
 ABI_PROBE_SOURCE = PACKAGE_DIR.parent / "tests" / "native" / "abi_probe.cpp"
 ABI_PROBE_PATH = PACKAGE_DIR.parent / "tests" / "native" / "abi_probe.bin"
-SOURCES = ("api.hip", "products.hip", "products_bf16.hip", "products_f16.hip", "products_i8.hip")
+SOURCES = ("api.hip", "products.hip", "products_f32.hip", "products_bf16.hip", "products_f16.hip", "products_i8.hip")
 
 # -packed-fp32-ops is switched off on purpose: the compiler must not fuse scalar fp32 code
 # into v_pk_* instructions on this target.

@@ -6,11 +6,14 @@
 
 namespace soapmi {
 // instantiated in the source files of their types
+extern template int row_products<ElemF32, KC>(hipStream_t, const RowProblem&, bool);
+extern template int row_products<ElemF32, XC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemBF16, KC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemBF16, XC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemF16, KC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemF16, XC>(hipStream_t, const RowProblem&, bool);
 extern template int row_products<ElemI8, KC>(hipStream_t, const RowProblem&, bool);
+extern template int sum_products<ElemF32>(hipStream_t, const SumProblem&, bool);
 extern template int sum_products<ElemBF16>(hipStream_t, const SumProblem&, bool);
 extern template int sum_products<ElemF16>(hipStream_t, const SumProblem&, bool);
 
@@ -40,9 +43,6 @@ namespace {
 
 constexpr int64_t kSizeLimit = (int64_t)1 << 30;
 
-using F32Tile = DefaultTile<float>::type;
-using F32Small = SmallTile<float>::type;
-
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int value_bytes(int dtype) { return dtype == kFloat32 ? 4 : 2; }
 
@@ -64,25 +64,6 @@ int check_sizes(const int64_t* ends, int64_t experts, int64_t tokens, int64_t n,
 // tile of up to `stored_rows` stored rows that fit the buffer descriptor.
 bool direct_ok(const void* base, int64_t ld_bytes, int64_t contiguous_bytes, int64_t stored_rows) {
   return aligned16(base) && ld_bytes % 16 == 0 && contiguous_bytes % 16 == 0 && ld_bytes * stored_rows < kBufferBytes / 2;
-}
-
-template <class Cfg>
-int launch_rows_f32(hipStream_t stream, RowProblem p, int k_contiguous, int vec_w, int vec_x) {
-  p.tiles_c = (int)ceil_div64(p.cols, Cfg::BM);
-  unsigned grid;
-  if (int rc = grid_of(most_row_tiles(p.groups, Cfg::BN) * p.tiles_c, &grid)) return rc;
-  hipLaunchKernelGGL((row_product_f32_kernel<Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p, k_contiguous, vec_w, vec_x);
-  SOAPMI_LAUNCH_CHECK();
-  return kOk;
-}
-
-template <class Cfg>
-int launch_sums_f32(hipStream_t stream, SumProblem p, int vec_dy, int vec_x) {
-  unsigned grid;
-  if (int rc = sum_grid(p, Cfg::BN, Cfg::BM, &grid)) return rc;
-  hipLaunchKernelGGL((sum_product_f32_kernel<Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p, vec_dy, vec_x);
-  SOAPMI_LAUNCH_CHECK();
-  return p.parts > 1 ? launch_join(stream, p) : kOk;
 }
 
 int check_gradient(int dtype, int out_dtype, const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
@@ -210,17 +191,9 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
   p.ldy = ldy;
   p.out_type = out_dtype;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == kFloat32) {
-    // (contiguous along: weights k, x the inner extent)
-    const int vec_w = aligned16(w) && ldw % 4 == 0 && k % 4 == 0 && (experts <= 1 || stride_w % 4 == 0);
-    const int vec_x = aligned16(x) && ldx % 4 == 0 && inner % 4 == 0;
-    const int64_t each = tokens / std::max<int64_t>(1, experts);
-    if (each <= 64 || prefer_small_tile<float>(tokens, cols, false))
-      return launch_rows_f32<F32Small>(s, p, transposed ? 0 : 1, vec_w, vec_x);
-    return launch_rows_f32<F32Tile>(s, p, transposed ? 0 : 1, vec_w, vec_x);
-  }
   const bool direct = direct_ok(x, p.ldr, inner * size, 256) && direct_ok(w, p.ldc, k * size, 256) &&
                       (experts <= 1 || p.stride_c % 16 == 0);
+  if (dtype == kFloat32) return transposed ? row_products<ElemF32, XC>(s, p, direct) : row_products<ElemF32, KC>(s, p, direct);
   if (dtype == kBFloat16) return transposed ? row_products<ElemBF16, XC>(s, p, direct) : row_products<ElemBF16, KC>(s, p, direct);
   return transposed ? row_products<ElemF16, XC>(s, p, direct) : row_products<ElemF16, KC>(s, p, direct);
 }
@@ -239,13 +212,8 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
   p.c = static_cast<const char*>(x);
   p.ldc = ldx * value_bytes(dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == kFloat32) {
-    const int vec_dy = aligned16(gradient) && ldg % 4 == 0 && n % 4 == 0;
-    const int vec_x = aligned16(x) && ldx % 4 == 0 && k % 4 == 0;
-    if (prefer_small_tile<float>(n * std::min<int64_t>(experts, 8), k, false)) return launch_sums_f32<F32Small>(s, p, vec_dy, vec_x);
-    return launch_sums_f32<F32Tile>(s, p, vec_dy, vec_x);
-  }
-  const bool direct = direct_ok(gradient, p.ldr, n * 2, 64) && direct_ok(x, p.ldc, k * 2, 64);
+  const bool direct = direct_ok(gradient, p.ldr, n * value_bytes(dtype), 64) && direct_ok(x, p.ldc, k * value_bytes(dtype), 64);
+  if (dtype == kFloat32) return sum_products<ElemF32>(s, p, direct);
   return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct) : sum_products<ElemF16>(s, p, direct);
 }
 

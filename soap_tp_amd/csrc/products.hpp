@@ -1,4 +1,4 @@
-// Products of a layer with weights grouped by expert, in 16-bit floating point and 8-bit integers.
+// Products of a layer with weights grouped by expert, in 32-bit and 16-bit floating point and 8-bit integers.
 //
 //   rows grouped (forward, input gradient):  Y[t, c] = sum_k R[t, k] C_e(t)[c, k]
 //   k grouped    (weight gradient):          D_e[r, c] = sum over t in e of R[t, r] C[t, c]
@@ -9,12 +9,12 @@
 // tile leave.  Nothing is read back to the host and no launch prepares another.
 //
 // Operands.  Each operand is KC (its k index is contiguous in memory) or XC (its row or column index
-// is).  A slab of 128 bytes of k (KC: 64 16-bit or 128 8-bit values; XC: 64 values) is kept in LDS
+// is).  A slab of 128 bytes of k (32, 64 or 128 values) is kept in LDS
 // twice, so that the next one travels while this one is multiplied:
 //   KC  S[x][128 bytes], 16-byte pieces, piece p of row x stored at p ^ key(x): the 16 rows that a
 //       fragment read touches then start in different banks;
-//   XC  S[k][x], 32-byte blocks, block b of row k stored at b ^ f(k); fragments are read with the
-//       transposing LDS read, which hands each lane 4 consecutive k of one x.
+//   XC  S[k][x], blocks of 16 values, block b of row k stored at b ^ f(k); fragments are read with the
+//       transposing LDS read, which hands each lane 4 consecutive k of one x (32-bit values: one by one).
 // Both layouts are linear in the order in which lanes fetch, which is what a load from memory straight
 // to LDS needs: the permutation is applied to the address each lane fetches from.
 //
@@ -22,8 +22,9 @@
 // consecutive columns of one output row; columns are dealt to fragments in such a way that two
 // fragments give a lane eight consecutive ones (one 16-byte store of 16-bit results).
 #pragma once
+#include <type_traits>
+
 #include "common.hpp"
-#include "gemm.hpp"
 
 namespace soapmi {
 
@@ -37,7 +38,6 @@ enum : int { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };  // SOAPMI_FLOAT32 ...
 struct ElemBF16 {
   static constexpr int SIZE = 2;
   using Acc = f32x4;
-  using Scalar = __bf16;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -45,15 +45,23 @@ struct ElemBF16 {
 struct ElemF16 {
   static constexpr int SIZE = 2;
   using Acc = f32x4;
-  using Scalar = _Float16;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+struct ElemF32 {
+  static constexpr int SIZE = 4;
+  using Acc = f32x4;
+  static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {  // four values of k, one after the other
+    const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(af[t], bf[t], c, 0, 0, 0);
+    return c;
   }
 };
 struct ElemI8 {
   static constexpr int SIZE = 1;
   using Acc = i32x4;
-  using Scalar = int8_t;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
   }
@@ -174,10 +182,12 @@ __device__ __forceinline__ bool locate_rows(const RowGroups& g, unsigned tiles_c
 __device__ __forceinline__ int kc_key(bool column_side, int x) {
   return column_side ? (x & 3) | ((x >> 1) & 4) : x & 7;
 }
-// ... and XC rows: a transposing read of 32 lanes covers k rows {0..3, 8..11} (+ 4).
-template <int BX>
+// ... and XC rows, whose blocks of 16 values change places: a transposing read of 32 lanes covers k rows
+// {0..3, 8..11} (+ 4); reads of single 32-bit values k rows {0, 4, 8, 12} (+ 1, 2, 3), of which two still
+// share banks (bit 3 would cost a lane a second offset; the matrix cores bound fp32 anyway).
+template <int SIZE, int BX>
 __device__ __forceinline__ int xc_key(int k) {
-  return ((k & 3) | ((k >> 1) & 4)) & (BX / 16 - 1);
+  return (SIZE == 4 ? k >> 2 & 1 : (k & 3) | ((k >> 1) & 4)) & (BX / 16 - 1);
 }
 
 // Columns of a wavefront's fragment i, row m of the matrix instruction: fragments 2i and 2i+1 give lane
@@ -246,18 +256,18 @@ __device__ __forceinline__ float exponent_value(int code) {  // 2^(code - 127); 
 // One operand of a tile: BX rows (or columns), slabs of 128 bytes (KC) or 64 values (XC) of k.
 template <class E, Layout L, Source S, int BX, int NT, bool COLUMN, int AHEAD>
 struct Loader {
-  static constexpr int SLAB_K = L == KC ? 128 / E::SIZE : 64;
-  static constexpr int BYTES = L == KC ? BX * 128 : 64 * BX * E::SIZE;
+  static constexpr int SLAB_K = 128 / E::SIZE;
+  static constexpr int BYTES = BX * 128;
   static constexpr int PIECES = BYTES / 16;
   static constexpr int NP = (PIECES + NT - 1) / NT;
-  static_assert(L == KC || E::SIZE == 2, "transposing reads are of 16-bit values");
+  static_assert(L == KC || E::SIZE >= 2, "8-bit operands are KC");
   static_assert(S != Direct || PIECES % 64 == 0, "whole wavefronts fetch");
   static constexpr int PER_ROW = L == KC ? 8 : BX * E::SIZE / 16;  // pieces in an LDS row
 
   // Piece q = tid + i * NT of an operand lies i * STEP stored rows below piece tid and in the same place of
   // its row, since the permutations look at row bits below STEP only.
   static constexpr int STEP = NT / PER_ROW;
-  static_assert(NP == 1 || STEP % 16 == 0, "one place in the row serves all of a lane's pieces");
+  static_assert(NP == 1 || STEP % (L == XC && E::SIZE == 4 ? 8 : 16) == 0, "one place in the row serves all of a lane's pieces");
 
   const char* base;
   int64_t ld;
@@ -273,7 +283,7 @@ struct Loader {
     row = q / PER_ROW;
     const int slot = q % PER_ROW;
     if (L == KC) piece = slot ^ kc_key(COLUMN, row);
-    else piece = (((slot >> 1) ^ xc_key<BX>(row)) << 1) | (slot & 1);
+    else piece = (slot / E::SIZE ^ xc_key<E::SIZE, BX>(row)) * E::SIZE | slot % E::SIZE;  // (SIZE pieces are 16 values)
   }
 
   __device__ __forceinline__ void init(const Operand& o, int tid_) {
@@ -289,16 +299,17 @@ struct Loader {
   }
 
   __device__ __forceinline__ const char* slab(int kt) const {
-    return L == KC ? base + (int64_t)kt * 128 : base + (int64_t)kt * 64 * ld;
+    return L == KC ? base + (int64_t)kt * 128 : base + (int64_t)kt * SLAB_K * ld;
   }
 
   // Direct: slab kt is sent piece by piece.  k_left = values of k from this slab on.  The buffer ends with
   // the last row's last value, so that rows behind it come as zeros; in a last slab that is cut short,
   // so do the pieces of a KC operand behind the cut.
   __device__ __forceinline__ void aim(int kt, int k_left) {
-    const int bytes = L == KC ? (valid - 1) * (int)ld + k_left * E::SIZE : (min(k_left, 64) - 1) * (int)ld + valid * E::SIZE;
+    const int k_here = min(k_left, SLAB_K);
+    const int bytes = L == KC ? (valid - 1) * (int)ld + k_here * E::SIZE : (k_here - 1) * (int)ld + valid * E::SIZE;
     resource = buffer_of(slab(kt), k_left > 0 ? bytes : 0);  // (behind the last slab: nothing but zeros)
-    offset_now = L == KC && first_piece * 16 >= k_left * E::SIZE ? kOutside : offset;
+    offset_now = L == KC && first_piece * 16 >= k_here * E::SIZE ? kOutside : offset;
   }
   __device__ __forceinline__ void send(int i, unsigned lds) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -316,7 +327,7 @@ struct Loader {
         const int r = min(row, valid - 1);  // rows behind the last one only reach results that are not stored
         at += r * ld;
         if (k_left >= SLAB_K) held[set][i] = load_bytes(at, 16);
-        else held[set][i] = load_bytes(at, k_left * E::SIZE - first_piece * 16);
+        else held[set][i] = load_bytes(at, max(k_left, 0) * E::SIZE - first_piece * 16);
       } else {
         at += row * ld;
         if (k_left >= SLAB_K && valid == BX) held[set][i] = load_bytes(at, 16);
@@ -339,19 +350,27 @@ struct Loader {
     if constexpr (L == KC) {
       const int x = x0 + (COLUMN ? column_of(i, m) : 16 * i + m);
       return *reinterpret_cast<const i32x4*>(lds + x * 128 + (((ks * 4 + g) ^ kc_key(COLUMN, x)) << 4));
-    } else {
+    } else if constexpr (E::SIZE == 2) {
       // lane m of a 16-lane group supplies four x (chunk m % 4) of k row m / 4 and receives column m
       const int x = x0 + (COLUMN ? 32 * (i >> 1) + 8 * (m & 3) + 4 * (i & 1) : 16 * i + 4 * (m & 3));
       i32x4 out;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = ks * 32 + g * 8 + h * 4 + (m >> 2);
-        char* p = const_cast<char*>(lds) + k * (BX * E::SIZE) + ((((x >> 4) ^ xc_key<BX>(k)) << 5) | ((x & 15) << 1));
-        const s16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)p);
+        char* p = const_cast<char*>(lds) + k * (BX * 2) + ((((x >> 4) ^ xc_key<2, BX>(k)) << 5) | ((x & 15) << 1));
+        const s16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
         const auto two = __builtin_bit_cast(int __attribute__((ext_vector_type(2))), part);
         out[2 * h] = two[0];
         out[2 * h + 1] = two[1];
+      }
+      return out;
+    } else {
+      const int x = x0 + (COLUMN ? column_of(i, m) : 16 * i + m);
+      i32x4 out;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int k = ks * 16 + g * 4 + t;
+        out[t] = *reinterpret_cast<const int*>(lds + k * (BX * 4) + ((((x >> 4) ^ xc_key<4, BX>(k)) << 6) | ((x & 15) << 2)));
       }
       return out;
     }
@@ -910,56 +929,6 @@ __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
   o.rows = r.valid;
   o.cols = c.valid;
   store_tile<Cfg, Cfg::TR>(o, acc, Unscaled{}, lds);
-}
-
-// ---- fp32 ----------------------------------------------------------------------------------
-// The fp32 matrix product of gemm.hpp, tile by tile.  A row-major result is the column-major transposed
-// one, so its M runs over the columns and its N over the rows here.
-
-template <class Cfg>
-__device__ __forceinline__ void f32_tile(const float* a, int64_t lda, int trans_a, const float* b, int64_t ldb, int trans_b,
-                                         int m, int n, int k, float* c, int64_t ldc, bool vec_a, bool vec_b, float* smem) {
-  GemmProblem<float> p;
-  p.A = a; p.B = b; p.lda = lda; p.ldb = ldb;
-  p.M = m; p.N = n; p.K = k;
-  p.transA = trans_a; p.transB = trans_b;
-  p.vecA = vec_a; p.vecB = vec_b;
-  p.tiles_m = p.tiles_n = p.num_tiles = 1;
-  p.lower = 0;
-  p.k_chunk = k > 0 ? k : 1;
-  p.ksel_b = nullptr;
-  EpiStore<float> store{c, ldc, 1.0f, 0.0f};
-  gemm_tile_body<float, Cfg, EpiStore<float>, -1>(p, store, 0, 0, smem);
-}
-
-template <class Cfg>
-__global__ __launch_bounds__(Cfg::NT) void row_product_f32_kernel(RowProblem p, int weights_k_contiguous, int vec_w, int vec_x) {
-  __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
-  RowTile tile;
-  int tile_c;
-  if (!locate_rows<Cfg::BN, Cfg::BN>(p.groups, p.tiles_c, blockIdx.x, tile, tile_c)) return;
-  const int c0 = tile_c * Cfg::BM;
-  const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
-  const float* w = reinterpret_cast<const float*>(p.c + (int64_t)tile.expert * p.stride_c) +
-                   (weights_k_contiguous ? (int64_t)c0 * ldc : (int64_t)c0);
-  const float* x = reinterpret_cast<const float*>(p.r) + (int64_t)tile.row * ldr;
-  float* y = static_cast<float*>(p.y) + (int64_t)tile.row * p.ldy + c0;
-  f32_tile<Cfg>(w, ldc, weights_k_contiguous, x, ldr, 0, min(Cfg::BM, p.cols - c0), tile.rows,
-                tile.expert >= p.groups.experts ? 0 : p.k, y, p.ldy, vec_w, vec_x, smem);
-}
-
-template <class Cfg>
-__global__ __launch_bounds__(Cfg::NT) void sum_product_f32_kernel(SumProblem p, int vec_dy, int vec_x) {
-  __shared__ __attribute__((aligned(16))) float smem[Cfg::LDS_ELEMS];
-  SumTile tile;
-  if (!locate_sum(p, blockIdx.x, tile)) return;
-  const int r0 = tile.tile_r * Cfg::BN, c0 = tile.tile_c * Cfg::BM;
-  const int64_t ldr = p.ldr / 4, ldc = p.ldc / 4;
-  const float* dy = reinterpret_cast<const float*>(p.r) + (int64_t)tile.begin * ldr + r0;
-  const float* x = reinterpret_cast<const float*>(p.c) + (int64_t)tile.begin * ldc + c0;
-  const Result o = sum_result(p, tile, r0, c0);
-  f32_tile<Cfg>(x, ldc, 0, dy, ldr, 1, min(Cfg::BM, p.cols - c0), min(Cfg::BN, p.rows - r0), tile.end - tile.begin,
-                static_cast<float*>(o.base), o.ld, vec_x, vec_dy, smem);
 }
 
 // ---- 8-bit codes ---------------------------------------------------------------------------

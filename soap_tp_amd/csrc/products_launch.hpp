@@ -1,5 +1,5 @@
 // Host side of products.hpp: which kernel a product runs on.  Each element type is instantiated in a
-// source file of its own (products_bf16.hip, products_f16.hip, products_i8.hip), which compile side by side.
+// source file of its own (products_f32.hip, products_bf16.hip, ...), which compile side by side.
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -44,16 +44,34 @@ int launch_few_rows(hipStream_t stream, RowProblem p) {
   return kOk;
 }
 
-// Microseconds that a product of `groups` experts' rows takes on tiles of br x bc, as measured on MI355X:
-// a slab of 128 bytes of k takes the compute unit `slab` us (`alone` if it has one workgroup only), and
-// a workgroup's start and end 3 us; units = workgroups that run at once.
-inline double tile_time(const RowGroups& g, int64_t cols, int64_t k_bytes, int br, int bc, double units, double slab, double alone) {
+// How long a compute unit takes for a slab (128 bytes of k) of a tile: us, measured on MI355X.  alone: with
+// one workgroup per compute unit and most of them idle.  At 16 and 8 bits the slabs' loads bound it; fp32
+// takes the matrix cores sixteen times as long as 16 bits take them.
+struct SlabTime {
+  double busy, alone;
+};
+template <class E, class Cfg>
+constexpr SlabTime slab_time() {
+  constexpr bool f32 = E::SIZE == 4;
+  if (Cfg::BR == WideTile::BR) return f32 ? SlabTime{8.4, 7.2} : SlabTime{1.50, 1.30};
+  if (Cfg::BR == MidTile::BR) return f32 ? SlabTime{2.1, 1.9} : SlabTime{0.60, 0.55};
+  return f32 ? SlabTime{1.2, 0.6} : SlabTime{0.62, 0.34};
+}
+// Workgroups that run at once.
+template <class Cfg>
+constexpr double units() {
+  return Cfg::BR == LowTile::BR ? 512 : 256;
+}
+
+template <class E, class Cfg>
+double row_time(const RowProblem& p) {
+  const RowGroups& g = p.groups;
   // (every expert's last tile is cut short: half a tile each, when nothing else is known)
-  const double rows = g.experts <= 1 ? (double)ceil_div64(g.tokens, br)
-                                     : std::max((double)std::min(g.experts, g.tokens), (double)g.tokens / br + 0.5 * g.experts);
-  const double tiles = rows * (double)ceil_div64(cols, bc), rounds = std::ceil(tiles / units);
-  const double each = tiles * 2 <= units ? alone : slab;
-  return 3.0 + rounds * each * (double)ceil_div64(k_bytes, 128);
+  const double rows = g.experts <= 1 ? (double)ceil_div64(g.tokens, Cfg::BR)
+                                     : std::max((double)std::min(g.experts, g.tokens), (double)g.tokens / Cfg::BR + 0.5 * g.experts);
+  const double tiles = rows * (double)ceil_div64(p.cols, Cfg::BC), rounds = std::ceil(tiles / units<Cfg>());
+  constexpr SlabTime slab = slab_time<E, Cfg>();
+  return 3.0 + rounds * (tiles * 2 <= units<Cfg>() ? slab.alone : slab.busy) * (double)ceil_div64((int64_t)p.k * E::SIZE, 128);
 }
 
 // Which tile.  Measured (bf16, us, low / mid / wide): 1024 rows, 1024 x 1024: 9.9 / 12.9 / 25.4; 2048 rows,
@@ -62,19 +80,15 @@ inline double tile_time(const RowGroups& g, int64_t cols, int64_t k_bytes, int b
 // 4096): 64 rows 12.1 against 12.8 of the low tile, 128 rows 19.3 against 13.1.
 template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
-  const int64_t k_bytes = (int64_t)p.k * E::SIZE;
-  const double low = tile_time(p.groups, p.cols, k_bytes, LowTile::BR, LowTile::BC, 512, 0.62, 0.34);
-  const double mid = tile_time(p.groups, p.cols, k_bytes, MidTile::BR, MidTile::BC, 256, 0.60, 0.55);
+  const double low = row_time<E, LowTile>(p), mid = row_time<E, MidTile>(p);
   if constexpr (LC == KC) {
     const double rows = (double)std::max<int64_t>(std::min(p.groups.experts, p.groups.tokens), ceil_div64(p.groups.tokens, FewTile::BR));
     const double each = std::min(32.0, (double)p.groups.tokens / rows);
-    const double few = 4.0 + rows * (double)ceil_div64(p.cols, FewTile::BC) * (32.0 + each) * (double)k_bytes / 9.3e6;
-    if (few < std::min(low, mid)) return launch_few_rows<E>(stream, p);
+    const double bytes = rows * (double)ceil_div64(p.cols, FewTile::BC) * (32.0 + each) * p.k * E::SIZE;
+    if (4.0 + bytes / 9.3e6 < std::min(low, mid)) return launch_few_rows<E>(stream, p);
   }
-  if constexpr (S == Direct) {
-    const double wide = tile_time(p.groups, p.cols, k_bytes, WideTile::BR, WideTile::BC, 256, 1.50, 1.30);
-    if (wide < std::min(low, mid)) return launch_rows<E, LC, S, WideTile>(stream, p);
-  }
+  if constexpr (S == Direct)
+    if (row_time<E, WideTile>(p) < std::min(low, mid)) return launch_rows<E, LC, S, WideTile>(stream, p);
   return mid <= low ? launch_rows<E, LC, S, MidTile>(stream, p) : launch_rows<E, LC, S, LowTile>(stream, p);
 }
 
@@ -86,7 +100,7 @@ int row_products(hipStream_t stream, const RowProblem& p, bool direct) {
 
 // Parts that the experts' rows are cut into when the tiles (of 128 x 128) fill less than half of the 256
 // compute units and the sums are long: as many as fill them, of 8 slabs of 64 rows at least.  65536 rows of
-// 512 x 512: PARTS_MEASURED.
+// 512 x 512, bf16: 530 us whole, 78 us in parts; 16384 rows of 1024 x 1024: 108 and 58.
 inline int sum_parts(int64_t experts, int64_t tokens, int64_t rows, int64_t cols) {
   const int64_t tiles = experts * ceil_div64(rows, 128) * ceil_div64(cols, 128);
   if (experts <= 0 || tiles <= 0 || tiles > 128) return 1;
@@ -115,13 +129,23 @@ int launch_sums(hipStream_t stream, SumProblem p) {
   return p.parts > 1 ? launch_join(stream, p) : kOk;
 }
 
-// Wide tiles from 192 of them on: SUMS_MEASURED
+// A tile's start, its first loads and its stores, which are what short sums consist of, take `ends` us more.
+template <class E, class Cfg>
+double sum_time(const SumProblem& p, double ends) {
+  const double tiles = (double)p.groups.experts * p.parts * (double)(ceil_div64(p.rows, Cfg::BR) * ceil_div64(p.cols, Cfg::BC));
+  const double slabs = std::max(1.0, (double)p.groups.tokens * E::SIZE / 128 / std::max(1, p.groups.experts * p.parts));
+  constexpr SlabTime slab = slab_time<E, Cfg>();
+  return std::ceil(tiles / units<Cfg>()) * (ends + slabs * (tiles * 2 <= units<Cfg>() ? slab.alone : slab.busy));
+}
+
+// Measured (bf16, us, mid / wide): 8192 rows, 4096 x 4096: 297 / 208; 8 experts of 2048 x 4096, 8192 rows:
+// 250 / 165; 5 experts of 520 x 1000, 1020 rows: 11.2 / 17.8; 32 experts of 512 x 512, 64 rows: 14.5 / 17.5.
 template <class E, Source S>
 int launch_sums(hipStream_t stream, const SumProblem& p) {
-  const int64_t wide_tiles = ceil_div64(p.rows, 256) * ceil_div64(p.cols, 256) * p.groups.experts;
+  const double low = sum_time<E, LowTile>(p, 3.0), mid = sum_time<E, MidTile>(p, 4.0);
   if constexpr (S == Direct)
-    if (wide_tiles >= 96 && p.parts == 1) return launch_sums<E, S, WideTile>(stream, p);
-  return launch_sums<E, S, MidTile>(stream, p);
+    if (sum_time<E, WideTile>(p, 10.0) < std::min(low, mid)) return launch_sums<E, S, WideTile>(stream, p);
+  return mid <= low ? launch_sums<E, S, MidTile>(stream, p) : launch_sums<E, S, LowTile>(stream, p);
 }
 
 // D_e = sums over the experts' rows.  direct: the operands may be fetched straight to LDS.

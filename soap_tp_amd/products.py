@@ -263,10 +263,15 @@ def expert_weight_gradient(
     if saved:
         # (restored for this product alone: expanding the codes inside the product kernel, tile by tile, was
         # slower than reading the matrix once more)
-        values = restore_activations(x)
+        values = torch.empty((tokens, inputs), dtype=dtype, device=gradient.device)
+        if values.numel():
+            _launch(index, "soapmi_restore_activations", code, x.codes.data_ptr(), _row_stride(x.codes), exponents.data_ptr(),
+                    _row_stride(exponents), tokens, inputs, values.data_ptr(), inputs)
     gradient, ldg = _rows(gradient)
     values, ldx = _rows(values)
-    nbytes = native_library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, outputs, inputs)
+    nbytes = 0  # (sums of under 1024 rows are never cut into parts)
+    if tokens >= 1024 * experts:
+        nbytes = native_library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, outputs, inputs)
     work = scratch(nbytes, gradient.device) if nbytes else None
     _launch(index, "soapmi_expert_weight_gradient", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx, pointer, experts,
             tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out), out.stride(0) if experts > 1 else 0,
