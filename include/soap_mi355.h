@@ -201,7 +201,9 @@ int soapmi_col_major_to_row_major_f32(const float* in, int64_t ldi, float* out, 
  * expert e's starts e * stride elements after the first.  `dtype` and `out_dtype` are one of the
  * SOAPMI_FLOAT32, SOAPMI_BFLOAT16, SOAPMI_FLOAT16; sums are formed in fp32 on the matrix cores (8-bit
  * codes: exactly, in 32-bit integers) and rounded once.  Results do not depend on scheduling.
- * tokens, n, k < 2^30.  Buffers of one call must not overlap, except where it says so. */
+ * tokens, n, k < 2^30.  Buffers of one call must not overlap.  Where an operand's rows start at multiples
+ * of 16 bytes, they are read in whole pieces of 16 bytes: what stands behind a row's last value in its
+ * last piece is read, and does not matter. */
 #define SOAPMI_FLOAT32 0
 #define SOAPMI_BFLOAT16 1
 #define SOAPMI_FLOAT16 2

@@ -60,10 +60,10 @@ int check_sizes(const int64_t* ends, int64_t experts, int64_t tokens, int64_t n,
   return kOk;
 }
 
-// Whether an operand can be fetched straight to LDS: whole, aligned 16-byte pieces, and offsets inside a
-// tile of up to `stored_rows` stored rows that fit the buffer descriptor.
-bool direct_ok(const void* base, int64_t ld_bytes, int64_t contiguous_bytes, int64_t stored_rows) {
-  return aligned16(base) && ld_bytes % 16 == 0 && contiguous_bytes % 16 == 0 && ld_bytes * stored_rows < kBufferBytes / 2;
+// Whether an operand can be fetched straight to LDS: rows that start at multiples of 16 bytes, and offsets
+// inside a tile of up to `stored_rows` stored rows that fit the buffer descriptor.
+bool direct_ok(const void* base, int64_t ld_bytes, int64_t stored_rows) {
+  return aligned16(base) && ld_bytes % 16 == 0 && ld_bytes * stored_rows < kBufferBytes / 2;
 }
 
 int check_gradient(int dtype, int out_dtype, const int64_t* ends, int64_t experts, int64_t tokens, int64_t n, int64_t k,
@@ -175,7 +175,7 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
   const int64_t inner = transposed ? n : k, cols = transposed ? k : n;
   SOAPMI_REQUIRE(ldx >= inner && ldw >= k && ldy >= cols, "leading dimensions are too small");
   SOAPMI_REQUIRE(stride_w >= 0, "stride_w must be non-negative");
-  if (tokens == 0 || cols == 0) return kOk;
+  if (tokens == 0 || cols == 0 || (experts == 0 && !zero_rest)) return kOk;
   SOAPMI_REQUIRE(y && (experts == 0 || inner == 0 || (x && w)), "buffer addresses must be nonzero");
   const int size = value_bytes(dtype);
   RowProblem p = {};
@@ -191,7 +191,7 @@ int soapmi_expert_product(int dtype, const void* x, int64_t ldx, const void* w, 
   p.ldy = ldy;
   p.out_type = out_dtype;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool direct = direct_ok(x, p.ldr, inner * size, 256) && direct_ok(w, p.ldc, k * size, 256) &&
+  const bool direct = direct_ok(x, p.ldr, 256) && direct_ok(w, p.ldc, 256) &&
                       (experts <= 1 || p.stride_c % 16 == 0);
   if (dtype == kFloat32) return transposed ? row_products<ElemF32, XC>(s, p, direct) : row_products<ElemF32, KC>(s, p, direct);
   if (dtype == kBFloat16) return transposed ? row_products<ElemBF16, XC>(s, p, direct) : row_products<ElemBF16, KC>(s, p, direct);
@@ -212,7 +212,7 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
   p.c = static_cast<const char*>(x);
   p.ldc = ldx * value_bytes(dtype);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool direct = direct_ok(gradient, p.ldr, n * value_bytes(dtype), 64) && direct_ok(x, p.ldc, k * value_bytes(dtype), 64);
+  const bool direct = direct_ok(gradient, p.ldr, 64) && direct_ok(x, p.ldc, 64);
   if (dtype == kFloat32) return sum_products<ElemF32>(s, p, direct);
   return dtype == kBFloat16 ? sum_products<ElemBF16>(s, p, direct) : sum_products<ElemF16>(s, p, direct);
 }
@@ -275,7 +275,7 @@ int soapmi_int8_product(const int8_t* codes, int64_t ldq, const float* scales, c
   p.out_type = out_dtype;
   p.token_scale = scales;
   p.channel_scale = w_scales;
-  const bool direct = direct_ok(codes, ldq, k, 256) && direct_ok(w_codes, ldw, k, 256);
+  const bool direct = direct_ok(codes, ldq, 256) && direct_ok(w_codes, ldw, 256);
   return row_products<ElemI8, KC>(static_cast<hipStream_t>(stream), p, direct);
 }
 

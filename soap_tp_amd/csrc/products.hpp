@@ -195,8 +195,8 @@ __device__ __forceinline__ int xc_key(int k) {
 __device__ __forceinline__ int column_of(int i, int m) { return 32 * (i >> 1) + 8 * (m >> 2) + 4 * (i & 1) + (m & 3); }
 
 enum Layout { KC, XC };
-// How an operand gets to LDS.  Direct: 16-byte pieces straight from memory (aligned operands).  Staged:
-// through registers, any alignment and size.
+// How an operand gets to LDS.  Direct: 16-byte pieces straight from memory (rows that start at multiples of
+// 16 bytes).  Staged: through registers, any alignment.
 enum Source { Direct, Staged };
 
 struct Operand {
@@ -303,12 +303,14 @@ struct Loader {
   }
 
   // Direct: slab kt is sent piece by piece.  k_left = values of k from this slab on.  The buffer ends with
-  // the last row's last value, so that rows behind it come as zeros; in a last slab that is cut short,
-  // so do the pieces of a KC operand behind the cut.
+  // the 16 bytes that hold the last row's last value (rows start at multiples of 16 bytes, so these are in
+  // one row and one page), so that rows behind the last one come as zeros.  In a last slab that is cut
+  // short, so do the pieces of a KC operand behind the cut; what the piece with the cut brings from behind
+  // it, trim() takes out again.
   __device__ __forceinline__ void aim(int kt, int k_left) {
     const int k_here = min(k_left, SLAB_K);
     const int bytes = L == KC ? (valid - 1) * (int)ld + k_here * E::SIZE : (k_here - 1) * (int)ld + valid * E::SIZE;
-    resource = buffer_of(slab(kt), k_left > 0 ? bytes : 0);  // (behind the last slab: nothing but zeros)
+    resource = buffer_of(slab(kt), k_left > 0 ? (bytes + 15) & ~15 : 0);  // (behind the last slab: nothing but zeros)
     offset_now = L == KC && first_piece * 16 >= k_here * E::SIZE ? kOutside : offset;
   }
   __device__ __forceinline__ void send(int i, unsigned lds) {
@@ -341,6 +343,22 @@ struct Loader {
     const int q = tid + i * NT;
     if constexpr (S == Staged)
       if (PIECES % NT == 0 || q < PIECES) *reinterpret_cast<i32x4*>(lds + q * 16) = held[set][i];
+  }
+
+  // The slab in LDS without the bytes of k from `left` on that are in the same piece as the one before them.
+  static __device__ __forceinline__ void trim(char* lds, int left, int tid) {
+    if constexpr (L == KC) {
+      for (int x = tid; x < BX; x += NT) {
+        i32x4* at = reinterpret_cast<i32x4*>(lds + x * 128 + ((left >> 4 ^ kc_key(COLUMN, x)) << 4));
+        i32x4 v = *at;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int keep = min(max((left & 15) - 4 * d, 0), 4);
+          v[d] = keep == 4 ? v[d] : v[d] & ((1 << (8 * keep)) - 1);
+        }
+        *at = v;
+      }
+    }
   }
 
   // 16 bytes of fragment data for (x, k step ks): KC: k pieces 4 ks + lane group; XC: 8 k values.
@@ -522,7 +540,16 @@ struct TileProduct {
       for (int set = 0; set < AHEAD; ++set)
         if (kt + set + 1 < slabs) slab(kt + set, set);
     }
-    const char* last = lds + stage_of(slabs - 1);
+    char* last = lds + stage_of(slabs - 1);
+    if (DIRECT && (LR == KC || LC == KC) && ((unsigned)k_count * E::SIZE & 15)) {
+      const int left = (k_count - (slabs - 1) * SLAB_K) * E::SIZE;
+      LoadR::trim(last, left, tid);
+      LoadC::trim(last + LoadR::BYTES, left, tid);
+      wait_lds();
+      barrier();
+#pragma unroll
+      for (int n = 0; n < READS; ++n) read(f0, n, last, wr0, wc0, 0, lane);
+    }
 #pragma unroll
     for (int n = 0; n < READS; ++n) read(f1, n, last, wr0, wc0, 1, lane);
 #pragma unroll

@@ -53,9 +53,9 @@ struct SlabTime {
 template <class E, class Cfg>
 constexpr SlabTime slab_time() {
   constexpr bool f32 = E::SIZE == 4;
-  if (Cfg::BR == WideTile::BR) return f32 ? SlabTime{8.4, 7.2} : SlabTime{1.50, 1.30};
-  if (Cfg::BR == MidTile::BR) return f32 ? SlabTime{2.1, 1.9} : SlabTime{0.60, 0.55};
-  return f32 ? SlabTime{1.2, 0.6} : SlabTime{0.62, 0.34};
+  if (Cfg::BR == WideTile::BR) return f32 ? SlabTime{7.2, 7.2} : SlabTime{1.50, 1.30};
+  if (Cfg::BR == MidTile::BR) return f32 ? SlabTime{1.9, 1.9} : SlabTime{0.60, 0.55};
+  return f32 ? SlabTime{1.05, 0.75} : SlabTime{0.62, 0.34};
 }
 // Workgroups that run at once.
 template <class Cfg>

@@ -184,6 +184,34 @@ def test_strides_and_alignment(device, dtype, pad, offset):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(150, 3, 131, 141), (40, 2, 7, 9), (300, 1, 259, 66), (3700, 2, 3603, 75)], ids=str)
+def test_aligned_rows_of_odd_length(device, shape, dtype):
+    """Rows that start at multiples of 16 bytes and end anywhere: what stands between a row's end and the
+    next one's start (here NaN) reaches nothing."""
+    tokens, experts, outputs, inputs = shape
+
+    def padded(seed, *size):
+        store = torch.full((*size[:-1], -(-size[-1] // 8) * 8), float("nan"), dtype=dtype, device=device)
+        store[..., :size[-1]] = values(device, seed, *size, dtype=dtype)
+        return store[..., :size[-1]]
+
+    x, weights, dy = padded(1, tokens, inputs), padded(2, experts, outputs, inputs), padded(3, tokens, outputs)
+    check_layer(device, dtype, *shape, seed=sum(shape), x=x, weights=weights, dy=dy)
+
+
+@pytest.mark.parametrize("tokens,outputs,inputs", [(40, 70, 141), (130, 200, 1090), (700, 260, 33), (3700, 3603, 75)])
+def test_int8_product_of_aligned_rows_of_odd_length(device, tokens, outputs, inputs):
+    generator = torch.Generator(device=device).manual_seed(inputs)
+    pair = []
+    for rows in (tokens, outputs):
+        store = torch.randint(-128, 128, (rows, -(-inputs // 16) * 16), generator=generator, device=device, dtype=torch.int8)
+        pair.append(store[:, :inputs])
+    one = torch.ones(max(tokens, outputs), device=device)
+    y = products.int8_product(pair[0], one[:tokens], pair[1], one[:outputs], out_dtype=torch.float32)
+    assert torch.equal(y.double(), torch.mm(pair[0].double(), pair[1].double().t()))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_other_orders(device, dtype):
     """Column-major inputs, rows and experts that are the same memory."""
     x, weights, dy, spans, ends = check_layer(device, dtype, 90, 2, 40, 48, seed=33)
@@ -227,6 +255,8 @@ def test_empty_extents(device, dtype):
     assert products.expert_product(empty(5, 8), empty(2, 0, 8), ends).shape == (5, 0)
     assert products.expert_weight_gradient(empty(5, 4), empty(5, 0), ends).shape == (2, 4, 0)
     none = torch.zeros(0, dtype=torch.int64, device=device)
+    kept = torch.full((5, 4), 7.0, dtype=dtype, device=device)
+    assert (products.expert_product(empty(5, 8) + 1, empty(0, 4, 8), none, out=kept) == 7).all()
     assert not products.expert_product(empty(5, 8) + 1, empty(0, 4, 8), none).any()
     assert products.expert_weight_gradient(empty(5, 4), empty(5, 8), none).shape == (0, 4, 8)
 
