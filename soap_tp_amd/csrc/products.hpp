@@ -233,6 +233,10 @@ template <int N>
 __device__ __forceinline__ void wait_loads() {  // all but the last N loads of this wavefront are done
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
+// Memory accesses stay on their side of this in the program.  A wavefront's LDS accesses are carried out in
+// order, so that is all that lanes of one wavefront need to hand each other values; without it the compiler,
+// which sees each lane by itself, may exchange a read and a write that belong to different lanes.
+__device__ __forceinline__ void keep_order() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
@@ -621,7 +625,7 @@ struct TokenChannel {
 };
 
 // A wavefront's results go through its share of LDS, so that it stores whole rows of its part of the tile
-// (64 bytes and more) instead of 16 bytes here and there.  Only its own accesses order these, no barrier.
+// (64 bytes and more) instead of 16 bytes here and there.  No other wavefront's share is touched: no barrier.
 constexpr int kStoreBytes = 8192;  // of LDS for each wavefront
 
 template <class Cfg, class Out, int A, class Acc, class Scale>
@@ -655,6 +659,7 @@ __device__ __forceinline__ void store_tile_as(const Result& o, const Acc (&acc)[
         }
       }
     }
+    keep_order();
     constexpr int ROWS = 64 / PIECES;  // of one store
 #pragma unroll
     for (int s = 0; s < AT_ONCE * 16 / ROWS; ++s) {
@@ -674,6 +679,7 @@ __device__ __forceinline__ void store_tile_as(const Result& o, const Acc (&acc)[
           if (c + q < o.cols) to[q] = v[q];
       }
     }
+    keep_order();
   }
 }
 

@@ -232,6 +232,22 @@ def test_results_in_float32_and_in_the_inputs_type(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("outputs", [3603, 3650, 3720])
+def test_every_result_is_its_own_row_and_column(device, dtype, outputs):
+    """Each result names its place: on the widest tiles, in both result types, with columns cut short."""
+    tokens, inputs = 3840, 64
+    x = torch.zeros(tokens, inputs, dtype=dtype, device=device)
+    w = torch.zeros(outputs, inputs, dtype=dtype, device=device)
+    rows, columns = torch.arange(tokens, device=device), torch.arange(outputs, device=device)
+    x[:, 0], x[:, 1], x[:, 2] = (rows // 64).to(dtype), (rows % 64).to(dtype), 1
+    w[:, 0], w[:, 1], w[:, 2], w[:, 3] = 64, 1, (columns % 128 / 128).to(dtype), 0
+    expected = rows[:, None].double() + (columns % 128).double() / 128
+    out = torch.zeros(tokens, outputs, device=device)
+    assert torch.equal(products.expert_product(x, w, None, out=out).double(), expected)
+    assert torch.equal(products.expert_product(x, w, None), out.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_dense_layer(device, dtype):
     x, w, dy = values(device, 1, 70, 136, dtype=dtype), values(device, 2, 48, 136, dtype=dtype), values(device, 3, 70, 48, dtype=dtype)
     one = torch.tensor([70], device=device)
