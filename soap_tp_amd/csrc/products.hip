@@ -109,14 +109,15 @@ template <class T>
 int launch_quantize(hipStream_t stream, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldq,
                     float* scales) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
-                      ldq * 64 < kBufferBytes;
-  // Long rows, and few rows, take a workgroup each; short ones a wavefront.
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
+  // Long rows take a workgroup each, short ones a wavefront.
+  const int64_t grid = cols > 1024 ? rows : ceil_div64(rows, 4);
+  SOAPMI_REQUIRE(grid * 256 < (int64_t)1 << 32, "the matrix has too many rows for one launch");
   if (cols > 1024)
-    hipLaunchKernelGGL((quantize_rows_kernel<T, 256>), dim3((unsigned)rows), dim3(256), 0, stream, x, ldx, (int)rows,
+    hipLaunchKernelGGL((quantize_rows_kernel<T, 256>), dim3((unsigned)grid), dim3(256), 0, stream, x, ldx, (int)rows,
                        (int)cols, vec_x, codes, ldq, vec_q, scales);
   else
-    hipLaunchKernelGGL((quantize_rows_kernel<T, 64>), dim3((unsigned)ceil_div64(rows, 4)), dim3(256), 0, stream, x, ldx,
+    hipLaunchKernelGGL((quantize_rows_kernel<T, 64>), dim3((unsigned)grid), dim3(256), 0, stream, x, ldx,
                        (int)rows, (int)cols, vec_x, codes, ldq, vec_q, scales);
   SOAPMI_LAUNCH_CHECK();
   return kOk;
@@ -126,11 +127,10 @@ template <class T>
 int launch_checkpoint(hipStream_t stream, const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes, int64_t ldq,
                       uint8_t* exponents, int64_t lde, int lowest) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
-                      ldq * 64 < kBufferBytes;
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
   const int64_t blocks = ceil_div64(cols, kCheckpointBlock);
   const int64_t grid = ceil_div64(rows * blocks, 16);
-  SOAPMI_REQUIRE(grid < (int64_t)1 << 31, "the matrix has too many blocks for one launch");
+  SOAPMI_REQUIRE(grid * 256 < (int64_t)1 << 32, "the matrix has too many blocks for one launch");
   hipLaunchKernelGGL((checkpoint_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, x, ldx, rows, (int)cols,
                      (int)blocks, vec_x, codes, ldq, vec_q, exponents, lde, lowest);
   SOAPMI_LAUNCH_CHECK();
@@ -141,11 +141,10 @@ template <class T>
 int launch_restore(hipStream_t stream, const int8_t* codes, int64_t ldq, const uint8_t* exponents, int64_t lde, int64_t rows,
                    int64_t cols, T* x, int64_t ldx) {
   const int vec_x = aligned16(x) && ldx * sizeof(T) % 16 == 0;
-  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0 &&
-                      ldq * 64 < kBufferBytes;
+  const int vec_q = reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ldq % 8 == 0;
   const int64_t pieces = ceil_div64(cols, 8);
   const int64_t grid = ceil_div64(rows * pieces, 256);
-  SOAPMI_REQUIRE(grid < (int64_t)1 << 31, "the matrix is too large for one launch");
+  SOAPMI_REQUIRE(grid * 256 < (int64_t)1 << 32, "the matrix is too large for one launch");
   hipLaunchKernelGGL((restore_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, codes, ldq, vec_q, exponents, lde, rows,
                      (int)cols, (int)pieces, x, ldx, vec_x);
   SOAPMI_LAUNCH_CHECK();

@@ -9,8 +9,8 @@
 // tile leave.  Nothing is read back to the host and no launch prepares another.
 //
 // Operands.  Each operand is KC (its k index is contiguous in memory) or XC (its row or column index
-// is).  A slab of 128 bytes of k (32, 64 or 128 values) is kept in LDS
-// twice, so that the next one travels while this one is multiplied:
+// is).  LDS holds two or four slabs of 128 bytes of k (32, 64 or 128 values), so that the next ones travel
+// while one is multiplied:
 //   KC  S[x][128 bytes], 16-byte pieces, piece p of row x stored at p ^ key(x): the 16 rows that a
 //       fragment read touches then start in different banks;
 //   XC  S[k][x], blocks of 16 values, block b of row k stored at b ^ f(k); fragments are read with the

@@ -12,9 +12,10 @@ using WideTile = ProductTile<256, 256, 2, 4, 2, 1>;
 using MidTile = ProductTile<128, 128, 2, 4, 4, 3>;
 using LowTile = ProductTile<32, 128, 1, 4, 4, 3>;
 
-inline int grid_of(int64_t tiles, unsigned* grid) {
-  const int64_t g = 8 * ((tiles + 7) / 8);
-  SOAPMI_REQUIRE(g < (int64_t)1 << 31, "the product has too many tiles for one launch");
+// Workgroups for `tiles` tiles, dealt to the 8 XCDs.  (A launch has fewer than 2^32 threads.)
+inline int grid_of(int64_t tiles, int threads, unsigned* grid) {
+  const int64_t g = 8 * ceil_div64(tiles, 8);
+  SOAPMI_REQUIRE(g * threads < (int64_t)1 << 32, "the product has too many tiles for one launch");
   *grid = (unsigned)g;
   return kOk;
 }
@@ -28,7 +29,7 @@ template <class E, Layout LC, Source S, class Cfg>
 int launch_rows(hipStream_t stream, RowProblem p) {
   p.tiles_c = (int)ceil_div64(p.cols, Cfg::BC);
   unsigned grid;
-  if (int rc = grid_of(most_row_tiles(p.groups, Cfg::BR) * p.tiles_c, &grid)) return rc;
+  if (int rc = grid_of(most_row_tiles(p.groups, Cfg::BR) * p.tiles_c, Cfg::NT, &grid)) return rc;
   hipLaunchKernelGGL((row_product_kernel<E, LC, S, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return kOk;
@@ -38,7 +39,7 @@ template <class E>
 int launch_few_rows(hipStream_t stream, RowProblem p) {
   p.tiles_c = (int)ceil_div64(p.cols, FewTile::BC);
   unsigned grid;
-  if (int rc = grid_of(most_row_tiles(p.groups, FewTile::BR) * p.tiles_c, &grid)) return rc;
+  if (int rc = grid_of(most_row_tiles(p.groups, FewTile::BR) * p.tiles_c, FewTile::NT, &grid)) return rc;
   hipLaunchKernelGGL((few_rows_kernel<E>), dim3(grid), dim3(FewTile::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return kOk;
@@ -113,17 +114,13 @@ inline size_t sum_partials_bytes(int64_t experts, int64_t tokens, int64_t rows, 
 
 int launch_join(hipStream_t stream, const SumProblem& p);  // products.hip
 
-// Workgroups of a launch whose tiles are br x bc.
-inline int sum_grid(SumProblem& p, int br, int bc, unsigned* grid) {
-  p.tiles_r = (int)ceil_div64(p.rows, br);
-  p.tiles_c = (int)ceil_div64(p.cols, bc);
-  return grid_of(8 * ceil_div64((int64_t)p.tiles_r * p.tiles_c, 8) * p.groups.experts * p.parts, grid);
-}
-
 template <class E, Source S, class Cfg>
 int launch_sums(hipStream_t stream, SumProblem p) {
+  p.tiles_r = (int)ceil_div64(p.rows, Cfg::BR);
+  p.tiles_c = (int)ceil_div64(p.cols, Cfg::BC);
   unsigned grid;
-  if (int rc = sum_grid(p, Cfg::BR, Cfg::BC, &grid)) return rc;
+  const int64_t tiles = 8 * ceil_div64((int64_t)p.tiles_r * p.tiles_c, 8);  // of a matrix
+  if (int rc = grid_of(tiles * p.groups.experts * p.parts, Cfg::NT, &grid)) return rc;
   hipLaunchKernelGGL((sum_product_kernel<E, S, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return p.parts > 1 ? launch_join(stream, p) : kOk;

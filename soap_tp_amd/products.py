@@ -135,6 +135,21 @@ def _spans(tensor: Tensor) -> Tuple[int, int]:
     return first, first + (reach + 1) * tensor.element_size()
 
 
+def _apart(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors share no element: their memory does not meet, or they are different columns of
+    rows with the same stride."""
+    (first, last), (low, high) = _spans(a), _spans(b)
+    if last <= low or high <= first:
+        return True
+    if a.ndim != 2 or b.ndim != 2 or a.stride(1) != 1 or b.stride(1) != 1:
+        return False
+    stride = a.stride(0) * a.element_size()
+    if stride <= 0 or stride != b.stride(0) * b.element_size():
+        return False
+    shift = (low - first) % stride
+    return shift >= a.size(1) * a.element_size() and stride - shift >= b.size(1) * b.element_size()
+
+
 def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, ...], **inputs: Optional[Tensor]) -> int:
     """``out`` as a caller gave it: rows of contiguous values, written in place, apart from the inputs.
     The code of its type."""
@@ -149,12 +164,9 @@ def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, .
             raise ValueError("out must have contiguous rows that do not overlap.")
         if len(shape) == 3 and shape[0] > 1 and strides[0] < (shape[1] - 1) * _row_stride(out) + shape[2]:
             raise ValueError("out must have matrices that do not overlap.")
-        first, last = _spans(out)
         for name, tensor in inputs.items():
-            if tensor is not None and tensor.numel():
-                low, high = _spans(tensor)
-                if low < last and first < high:
-                    raise ValueError(f"out must not overlap {name}.")
+            if tensor is not None and tensor.numel() and not _apart(out, tensor):
+                raise ValueError(f"out must not overlap {name}.")
     return _DTYPES[out.dtype]
 
 

@@ -673,6 +673,38 @@ def test_captured_and_replayed(device, dtype):
             assert torch.equal(actual, expected)
 
 
+def test_long_sums_captured_and_replayed(device):
+    """Sums cut into parts, with the parts' memory from the graph's own pool."""
+    x, dy = (torch.empty(4000, n, dtype=torch.bfloat16, device=device) for n in (72, 136))
+
+    def fill(seed):
+        x.copy_(values(device, seed, 4000, 72, dtype=torch.bfloat16))
+        dy.copy_(values(device, seed + 1, 4000, 136, dtype=torch.bfloat16))
+
+    fill(0)
+    products.expert_weight_gradient(dy, x, None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = products.expert_weight_gradient(dy, x, None)
+    for seed in (5, 9):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, products.expert_weight_gradient(dy, x, None))
+
+
+def test_columns_of_one_buffer(device):
+    """A result written between the columns of its own input's buffer."""
+    buffer = torch.zeros(50, 24, dtype=torch.bfloat16, device=device)
+    buffer[:, :8] = values(device, 1, 50, 8, dtype=torch.bfloat16)
+    w = values(device, 2, 16, 8, dtype=torch.bfloat16)
+    expected = products.expert_product(buffer[:, :8].clone(), w, None)
+    kept = buffer[:, :8].clone()
+    products.expert_product(buffer[:, :8], w, None, out=buffer[:, 8:])
+    assert torch.equal(buffer[:, 8:], expected) and torch.equal(buffer[:, :8], kept)
+
+
 def test_two_streams_at_once_and_twice_the_same(device):
     x, weights = values(device, 1, 400, 256, dtype=torch.bfloat16), values(device, 2, 4, 192, 256, dtype=torch.bfloat16)
     dy = values(device, 3, 400, 192, dtype=torch.bfloat16)

@@ -52,6 +52,19 @@ def test_expert_product_refusals(arguments, message):
         products.expert_product(call["x"], call["weights"], call["ends"], out=call["out"])
 
 
+def test_overlap_is_that_of_elements():
+    """Different columns of one buffer are apart, however their memory interleaves."""
+    buffer = torch.zeros(6, 20)
+    a, b = buffer[:, :8], buffer[:, 8:20]
+    assert products._apart(a, b) and products._apart(b, a)
+    assert not products._apart(buffer[:, :9], b) and not products._apart(b, buffer[:, 4:9])
+    assert products._apart(buffer[:3], buffer[3:]) and not products._apart(buffer[:4], buffer[3:])
+    assert not products._apart(a, buffer.view(12, 10)[:, 8:])  # other strides that meet
+    assert not products._apart(buffer.t(), b)
+    with pytest.raises(ValueError, match="requires cuda buffers"):  # not "overlap"
+        products.expert_product(buffer[:, :8], torch.zeros(12, 8), None, out=buffer[:, 8:])
+
+
 def test_input_gradient_refusals():
     with pytest.raises(ValueError, match="gradient has 8 columns, expected 4"):
         products.expert_input_gradient(X, W, _ends(3, 6))
@@ -138,6 +151,8 @@ def test_checkpoint_and_int8_refusals():
     ("soapmi_checkpoint_activations", (0, None, 8, 6, 8, P, 8, P, 1, None), "nonzero"),
     ("soapmi_restore_activations", (7, P, 8, P, 1, 6, 8, P, 8, None), "dtype must be 0"),
     ("soapmi_quantize_rows", (0, P, 8, 6, 8, P, 7, P, None), "leading dimensions"),
+    ("soapmi_quantize_rows", (0, P, 2000, 1 << 25, 2000, P, 2000, P, None), "too many rows"),
+    ("soapmi_expert_product", (1, P, 8, P, 8, 64, 0, P, 1 << 20, 1 << 29, 1 << 20, 8, 1, P, 1 << 20, 0, None), "too many tiles"),
     ("soapmi_int8_product", (P, 131072, P, P, 131072, P, 6, 4, 131072, 1, P, 4, None), "at most 131071"),
     ("soapmi_int8_product", (P, 8, None, P, 8, P, 6, 4, 8, 1, P, 4, None), "nonzero"),
 ])
