@@ -324,7 +324,11 @@ def expert_linear(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, checkpo
 
     With ``checkpoint`` the input is kept for the backward pass in 8 bits (``checkpoint_activations``)
     instead of in its own type; the weights' gradient is then that of the restored input, ``x``'s
-    gradient and the result are unchanged."""
+    gradient and the result are unchanged.
+
+    To capture it with its backward pass into a graph, capture both together and let no earlier autograd
+    graph of the same leaves live: torch accumulates a leaf's gradient on the stream of the first graph that
+    holds the leaf, and a capture cannot wait for that stream."""
     return _ExpertLinear.apply(x, weights, ends, checkpoint)
 
 

@@ -694,6 +694,43 @@ def test_long_sums_captured_and_replayed(device):
         assert torch.equal(captured, products.expert_weight_gradient(dy, x, None))
 
 
+def test_training_pass_captured_and_replayed(device):
+    """Forward and backward pass through autograd in one graph, on other inputs and splits."""
+    tokens, experts, outputs, inputs = 150, 4, 40, 136
+    x, dy = (torch.zeros(tokens, n, dtype=torch.bfloat16, device=device) for n in (inputs, outputs))
+    weights = torch.zeros(experts, outputs, inputs, dtype=torch.bfloat16, device=device)
+    ends = torch.zeros(experts, dtype=torch.int64, device=device)
+    leaves = x.requires_grad_(), weights.requires_grad_()
+
+    def fill(seed):
+        with torch.no_grad():
+            x.copy_(values(device, seed, tokens, inputs, dtype=torch.bfloat16))
+            dy.copy_(values(device, seed + 1, tokens, outputs, dtype=torch.bfloat16))
+            weights.copy_(values(device, seed + 2, experts, outputs, inputs, dtype=torch.bfloat16))
+            ends.copy_(split(tokens, experts, device, seed, spare=seed)[1])
+
+    def eager():
+        with torch.no_grad():
+            saved = products.checkpoint_activations(x)
+            return (products.expert_product(x, weights, ends), products.expert_input_gradient(dy, weights, ends),
+                    products.expert_weight_gradient(dy, saved, ends, out_dtype=torch.bfloat16))
+
+    fill(0)
+    eager()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = products.expert_linear(x, weights, ends, checkpoint=True)
+        captured = torch.autograd.grad(y, leaves, dy)
+        y = y.detach()
+    for seed in (3, 11, 20):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        for actual, expected in zip((y, *captured), eager()):
+            assert torch.equal(actual, expected)
+
+
 def test_columns_of_one_buffer(device):
     """A result written between the columns of its own input's buffer."""
     buffer = torch.zeros(50, 24, dtype=torch.bfloat16, device=device)
