@@ -11,6 +11,7 @@ namespace soapmi {
 using WideTile = ProductTile<256, 256, 2, 4, 2, 1>;
 using MidTile = ProductTile<128, 128, 2, 4, 4, 3>;
 using LowTile = ProductTile<32, 128, 1, 4, 4, 3>;
+using SmallTile = ProductTile<32, 64, 2, 2, 4, 3>;  // fp32 rows straight from memory only
 
 // Workgroups for `tiles` tiles, dealt to the 8 XCDs.  (A launch has fewer than 2^32 threads.)
 inline int grid_of(int64_t tiles, int threads, unsigned* grid) {
@@ -55,13 +56,14 @@ template <class E, class Cfg>
 constexpr SlabTime slab_time() {
   constexpr bool f32 = E::SIZE == 4;
   if (Cfg::BR == WideTile::BR) return f32 ? SlabTime{7.2, 7.2} : SlabTime{1.50, 1.30};
+  if (Cfg::BC == SmallTile::BC) return SlabTime{0.85, 0.50};
   if (Cfg::BR == MidTile::BR) return f32 ? SlabTime{1.9, 1.9} : SlabTime{0.60, 0.55};
   return f32 ? SlabTime{1.05, 0.75} : SlabTime{0.62, 0.34};
 }
 // Workgroups that run at once.
 template <class Cfg>
 constexpr double units() {
-  return Cfg::BR == LowTile::BR ? 512 : 256;
+  return Cfg::BC == SmallTile::BC ? 768 : Cfg::BR == LowTile::BR ? 512 : 256;
 }
 
 template <class E, class Cfg>
@@ -79,17 +81,27 @@ double row_time(const RowProblem& p) {
 // 2048 x 2048: 35.5 / 22.6 / 42.6; 8 experts of 4096 x 4096 with 128 rows each: 115 / 69 / 97, with 384 each:
 // 251 / 134 / 107.  Few rows (32 outputs x 32 rows at a time, read from L2 at about 9.3 TB/s; bytes, 4096 x
 // 4096): 64 rows 12.1 against 12.8 of the low tile, 128 rows 19.3 against 13.1.
+// fp32 has the small tile as well: its matrix instructions take so long that few large tiles leave most of the
+// chip idle for long (input gradient, low / small / mid: 500 rows, 2048 x 512: 47.6 / 34.0 / 126; 100 rows, 1024 x
+// 1024: 26.4 / 19.1 / 65.9; 4 experts of 1024 x 1100, 1000 rows: 43.3 / 37.0 / 66.7; 1024 rows, 1024 x 1024:
+// 29.0 / 28.9 / 66.7; forward, 2048^3: 147 / 167 / 128).  At 16 bits, where the slabs' latency bounds small
+// products, it is no clear gain (low / small: 1024 rows, 1024 x 1024: 9.9 / 10.4; 256 rows: 9.3 / 8.4).
 template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
   const double low = row_time<E, LowTile>(p), mid = row_time<E, MidTile>(p);
+  constexpr bool has_small = S == Direct && E::SIZE == 4;
+  double best = std::min(low, mid), small = best;
+  if constexpr (has_small) best = std::min(best, small = row_time<E, SmallTile>(p));
   if constexpr (LC == KC) {
     const double rows = (double)std::max<int64_t>(std::min(p.groups.experts, p.groups.tokens), ceil_div64(p.groups.tokens, FewTile::BR));
     const double each = std::min(32.0, (double)p.groups.tokens / rows);
     const double bytes = rows * (double)ceil_div64(p.cols, FewTile::BC) * (32.0 + each) * p.k * E::SIZE;
-    if (4.0 + bytes / 9.3e6 < std::min(low, mid)) return launch_few_rows<E>(stream, p);
+    if (4.0 + bytes / 9.3e6 < best) return launch_few_rows<E>(stream, p);
   }
   if constexpr (S == Direct)
-    if (row_time<E, WideTile>(p) < std::min(low, mid)) return launch_rows<E, LC, S, WideTile>(stream, p);
+    if (row_time<E, WideTile>(p) < best) return launch_rows<E, LC, S, WideTile>(stream, p);
+  if constexpr (has_small)
+    if (small < std::min(low, mid)) return launch_rows<E, LC, S, SmallTile>(stream, p);
   return mid <= low ? launch_rows<E, LC, S, MidTile>(stream, p) : launch_rows<E, LC, S, LowTile>(stream, p);
 }
 

@@ -114,6 +114,12 @@ def test_long_sums_with_and_without_a_workspace(device, dtype):
         call(work.data_ptr(), need - 1)
 
 
+@pytest.mark.parametrize("shape", [(1000, 4, 1024, 1100), (530, 3, 516, 1028), (700, 1, 1030, 1028), (259, 40, 260, 132)], ids=str)
+def test_layer_products_in_single_precision(device, shape):
+    """Sizes between a handful of rows and full tiles, rows at multiples of 16 bytes and not."""
+    check_layer(device, torch.float32, *shape, seed=6, spare=5)
+
+
 @pytest.mark.parametrize("dtype", HALF, ids=str)
 @pytest.mark.parametrize("outputs,inputs", [(3600, 3584), (3601, 3590)], ids=str)
 def test_layer_products_on_the_widest_tiles(device, dtype, outputs, inputs):
