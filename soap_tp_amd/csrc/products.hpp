@@ -211,13 +211,18 @@ constexpr int kBufferBytes = 0x40000000;
 // 16 bytes per lane from memory (resource's address + offset + more) to LDS at lds + 16 * lane (more and lds:
 // the same in all lanes of a wavefront); zeros where the resource ends before them.
 // In inline assembly because the compiler, told of such a load, waits for it before every transposing
-// LDS read, the ones of the other buffer included.  There is no output register; the waits are
-// wait_arrived().
+// LDS read, the ones of the other buffer included.  There is no output but m0; wait_loads() waits for the load.
+// The compiler does not look inside for hazards either: a scalar register that a vector instruction wrote may be
+// read by a memory instruction five wait states later at the earliest, m0 one after a scalar write.  The s_nop
+// is for m0.  The other registers come from scalar instructions, or from long before, and the build refuses a
+// library where one does not (five wait states at every load instead: 8192^3 forward 762 -> 772 us, weight
+// gradient 758 -> 771; at every new resource: 773 -> 777, input gradient 759 -> 768).
 __device__ __forceinline__ void load_to_lds(i32x4 resource, unsigned offset, unsigned more, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
+  unsigned m0;
+  asm volatile("s_mov_b32 %0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds"
+               : "=&{m0}"(m0)
                : "s"(lds), "v"(offset), "s"(resource), "s"(more)
-               : "memory", "m0");
+               : "memory");
 }
 
 __device__ __forceinline__ i32x4 buffer_of(const char* base, int bytes) {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import soap_tp_amd
-from soap_tp_amd import _native, products
+from soap_tp_amd import _native, build, products
 
 P = 4096  # a non-null address that no refused call dereferences
 
@@ -172,3 +172,31 @@ def test_entry_points_refuse(name, arguments, message):
 ])
 def test_empty_results_need_no_buffers(name, arguments):
     _native.call(name, *arguments)
+
+
+LISTING = """
+0000000000001000 <kernel>:
+	s_load_dwordx2 s[0:1], s[4:5], 0x0                         // 000000001000: C0060002 00000000
+	v_readfirstlane_b32 s{written}, v1                         // 000000001008: 7E080501
+	{wait}                                                     // 00000000100C: BF800000
+	s_cbranch_scc1 {jump}                                      // 000000001010: BF850001
+	s_mov_b32 m0, s9                                           // 000000001014: BEFC0009
+	s_nop 0                                                    // 000000001018: BF800000
+	buffer_load_dwordx4 v2, s[0:3], s8 offen lds               // 00000000101C: E05D1000 08000002
+	s_endpgm                                                   // 000000001024: BF810000
+"""
+
+
+@pytest.mark.parametrize("written,wait,jump,found", [
+    (2, "s_nop 0", 4, 1), (8, "s_nop 0", 4, 1), (9, "s_nop 0", 4, 0), (2, "s_nop 1", 4, 0), (2, "s_nop 0", 65535, 1),
+    (2, "s_nop 1", 2, 1),  # straight to the load
+    (2, "s_nop 3", 2, 0),
+])
+def test_the_build_sees_a_load_that_does_not_wait(written, wait, jump, found):
+    """The loads to LDS written in assembly are out of the compiler's sight: five wait states have to pass between
+    a vector instruction that writes a scalar register and a memory instruction that reads it."""
+    assert len(build.unsettled_loads(LISTING.format(written=written, wait=wait, jump=jump))) == found
+
+
+def test_no_load_of_the_library_reads_a_register_too_soon():
+    assert build.check_loads(_native.LIBRARY_PATH) > 100
