@@ -13,11 +13,14 @@ using MidTile = ProductTile<128, 128, 2, 4, 4, 3>;
 using LowTile = ProductTile<32, 128, 1, 4, 4, 3>;
 using SmallTile = ProductTile<32, 64, 2, 2, 4, 3>;  // fp32 rows straight from memory only
 
-// Workgroups for `tiles` tiles, dealt to the 8 XCDs.  (A launch has fewer than 2^32 threads.)
+// Workgroups for `tiles` tiles, dealt to the 8 XCDs.
+inline int64_t workgroups_of(int64_t tiles) { return 8 * ceil_div64(tiles, 8); }
+// A launch has fewer than 2^32 threads.
+inline bool fits_launch(int64_t tiles, int threads) { return workgroups_of(tiles) * threads < (int64_t)1 << 32; }
+
 inline int grid_of(int64_t tiles, int threads, unsigned* grid) {
-  const int64_t g = 8 * ceil_div64(tiles, 8);
-  SOAPMI_REQUIRE(g * threads < (int64_t)1 << 32, "the product has too many tiles for one launch");
-  *grid = (unsigned)g;
+  SOAPMI_REQUIRE(fits_launch(tiles, threads), "the product has too many tiles for one launch");
+  *grid = (unsigned)workgroups_of(tiles);
   return kOk;
 }
 
@@ -26,11 +29,17 @@ inline int64_t most_row_tiles(const RowGroups& g, int br) {
   return g.tokens / br + std::min<int64_t>((int64_t)g.experts + g.rest, g.tokens);
 }
 
+// Tiles of a launch.
+template <class Cfg>
+int64_t row_tiles(const RowProblem& p) {
+  return most_row_tiles(p.groups, Cfg::BR) * ceil_div64(p.cols, Cfg::BC);
+}
+
 template <class E, Layout LC, Source S, class Cfg>
 int launch_rows(hipStream_t stream, RowProblem p) {
   p.tiles_c = (int)ceil_div64(p.cols, Cfg::BC);
   unsigned grid;
-  if (int rc = grid_of(most_row_tiles(p.groups, Cfg::BR) * p.tiles_c, Cfg::NT, &grid)) return rc;
+  if (int rc = grid_of(row_tiles<Cfg>(p), Cfg::NT, &grid)) return rc;
   hipLaunchKernelGGL((row_product_kernel<E, LC, S, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return kOk;
@@ -40,7 +49,7 @@ template <class E>
 int launch_few_rows(hipStream_t stream, RowProblem p) {
   p.tiles_c = (int)ceil_div64(p.cols, FewTile::BC);
   unsigned grid;
-  if (int rc = grid_of(most_row_tiles(p.groups, FewTile::BR) * p.tiles_c, FewTile::NT, &grid)) return rc;
+  if (int rc = grid_of(row_tiles<FewTile>(p), FewTile::NT, &grid)) return rc;
   hipLaunchKernelGGL((few_rows_kernel<E>), dim3(grid), dim3(FewTile::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return kOk;
@@ -66,8 +75,10 @@ constexpr double units() {
   return Cfg::BC == SmallTile::BC ? 768 : Cfg::BR == LowTile::BR ? 512 : 256;
 }
 
+// (no launch takes too many tiles, whatever the others take)
 template <class E, class Cfg>
 double row_time(const RowProblem& p) {
+  if (!fits_launch(row_tiles<Cfg>(p), Cfg::NT)) return HUGE_VAL;
   const RowGroups& g = p.groups;
   // (every expert's last tile is cut short: half a tile each, when nothing else is known)
   const double rows = g.experts <= 1 ? (double)ceil_div64(g.tokens, Cfg::BR)
@@ -75,6 +86,15 @@ double row_time(const RowProblem& p) {
   const double tiles = rows * (double)ceil_div64(p.cols, Cfg::BC), rounds = std::ceil(tiles / units<Cfg>());
   constexpr SlabTime slab = slab_time<E, Cfg>();
   return 3.0 + rounds * (tiles * 2 <= units<Cfg>() ? slab.alone : slab.busy) * (double)ceil_div64((int64_t)p.k * E::SIZE, 128);
+}
+
+// The same for few rows (see few_rows_kernel): their bytes, weights and rows, from L2.
+template <class E>
+double few_rows_time(const RowProblem& p) {
+  if (!fits_launch(row_tiles<FewTile>(p), FewTile::NT)) return HUGE_VAL;
+  const double rows = (double)std::max<int64_t>(std::min(p.groups.experts, p.groups.tokens), ceil_div64(p.groups.tokens, FewTile::BR));
+  const double each = std::min(32.0, (double)p.groups.tokens / rows);
+  return 4.0 + rows * (double)ceil_div64(p.cols, FewTile::BC) * (32.0 + each) * p.k * E::SIZE / 9.3e6;
 }
 
 // Which tile.  Measured (bf16, us, low / mid / wide): 1024 rows, 1024 x 1024: 9.9 / 12.9 / 25.4; 2048 rows,
@@ -88,18 +108,16 @@ double row_time(const RowProblem& p) {
 // products, it is no clear gain (low / small: 1024 rows, 1024 x 1024: 9.9 / 10.4; 256 rows: 9.3 / 8.4).
 template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
-  const double low = row_time<E, LowTile>(p), mid = row_time<E, MidTile>(p);
   constexpr bool has_small = S == Direct && E::SIZE == 4;
-  double best = std::min(low, mid), small = best;
-  if constexpr (has_small) best = std::min(best, small = row_time<E, SmallTile>(p));
-  if constexpr (LC == KC) {
-    const double rows = (double)std::max<int64_t>(std::min(p.groups.experts, p.groups.tokens), ceil_div64(p.groups.tokens, FewTile::BR));
-    const double each = std::min(32.0, (double)p.groups.tokens / rows);
-    const double bytes = rows * (double)ceil_div64(p.cols, FewTile::BC) * (32.0 + each) * p.k * E::SIZE;
-    if (4.0 + bytes / 9.3e6 < best) return launch_few_rows<E>(stream, p);
-  }
+  const double low = row_time<E, LowTile>(p), mid = row_time<E, MidTile>(p);
+  double few = HUGE_VAL, wide = HUGE_VAL, small = HUGE_VAL;
+  if constexpr (LC == KC) few = few_rows_time<E>(p);
+  if constexpr (S == Direct) wide = row_time<E, WideTile>(p);
+  if constexpr (has_small) small = row_time<E, SmallTile>(p);
+  if constexpr (LC == KC)
+    if (few < std::min({low, mid, wide, small})) return launch_few_rows<E>(stream, p);
   if constexpr (S == Direct)
-    if (row_time<E, WideTile>(p) < best) return launch_rows<E, LC, S, WideTile>(stream, p);
+    if (wide < std::min({low, mid, small})) return launch_rows<E, LC, S, WideTile>(stream, p);
   if constexpr (has_small)
     if (small < std::min(low, mid)) return launch_rows<E, LC, S, SmallTile>(stream, p);
   return mid <= low ? launch_rows<E, LC, S, MidTile>(stream, p) : launch_rows<E, LC, S, LowTile>(stream, p);
@@ -126,13 +144,17 @@ inline size_t sum_partials_bytes(int64_t experts, int64_t tokens, int64_t rows, 
 
 int launch_join(hipStream_t stream, const SumProblem& p);  // products.hip
 
+template <class Cfg>
+int64_t sum_tiles(const SumProblem& p) {  // (a matrix has a multiple of 8)
+  return workgroups_of(ceil_div64(p.rows, Cfg::BR) * ceil_div64(p.cols, Cfg::BC)) * p.groups.experts * p.parts;
+}
+
 template <class E, Source S, class Cfg>
 int launch_sums(hipStream_t stream, SumProblem p) {
   p.tiles_r = (int)ceil_div64(p.rows, Cfg::BR);
   p.tiles_c = (int)ceil_div64(p.cols, Cfg::BC);
   unsigned grid;
-  const int64_t tiles = 8 * ceil_div64((int64_t)p.tiles_r * p.tiles_c, 8);  // of a matrix
-  if (int rc = grid_of(tiles * p.groups.experts * p.parts, Cfg::NT, &grid)) return rc;
+  if (int rc = grid_of(sum_tiles<Cfg>(p), Cfg::NT, &grid)) return rc;
   hipLaunchKernelGGL((sum_product_kernel<E, S, Cfg>), dim3(grid), dim3(Cfg::NT), 0, stream, p);
   SOAPMI_LAUNCH_CHECK();
   return p.parts > 1 ? launch_join(stream, p) : kOk;
@@ -141,6 +163,7 @@ int launch_sums(hipStream_t stream, SumProblem p) {
 // A tile's start, its first loads and its stores, which are what short sums consist of, take `ends` us more.
 template <class E, class Cfg>
 double sum_time(const SumProblem& p, double ends) {
+  if (!fits_launch(sum_tiles<Cfg>(p), Cfg::NT)) return HUGE_VAL;
   const double tiles = (double)p.groups.experts * p.parts * (double)(ceil_div64(p.rows, Cfg::BR) * ceil_div64(p.cols, Cfg::BC));
   const double slabs = std::max(1.0, (double)p.groups.tokens * E::SIZE / 128 / std::max(1, p.groups.experts * p.parts));
   constexpr SlabTime slab = slab_time<E, Cfg>();

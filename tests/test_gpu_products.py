@@ -766,3 +766,16 @@ def test_two_streams_at_once_and_twice_the_same(device):
     for results in (*found[0], *found[1]):
         for actual, wanted in zip(results, expected):
             assert torch.equal(actual, wanted)
+
+
+@pytest.mark.parametrize("dtype,inputs", [(torch.bfloat16, 8), (torch.bfloat16, 9), (torch.float32, 16)], ids=str)
+def test_very_many_rows_of_short_products(device, dtype, inputs):
+    """More tiles of few rows than a launch can have: a larger tile takes them."""
+    tokens, outputs = 1 << 21, 4096
+    x, w = values(device, 1, tokens, inputs, dtype=dtype), values(device, 2, outputs, inputs, dtype=dtype)
+    y = products.expert_product(x, w, None)
+    for first in range(0, tokens, 1 << 17):
+        rows = slice(first, first + (1 << 17))
+        wide = torch.mm(x[rows].double(), w.double().t())
+        allowed = (inputs + 1) * 2.0 ** -23 * torch.mm(x[rows].double().abs(), w.double().abs().t())
+        assert ((y[rows].double() - wide).abs() <= allowed + rounding(wide.abs() + allowed, dtype)).all()

@@ -200,3 +200,19 @@ def test_the_build_sees_a_load_that_does_not_wait(written, wait, jump, found):
 
 def test_no_load_of_the_library_reads_a_register_too_soon():
     assert build.check_loads(_native.LIBRARY_PATH) > 100
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the launch has to fail for want of a GPU")
+@pytest.mark.parametrize("name,arguments", [
+    # rows, outputs, inputs: short inner sizes with many rows, on tiles straight from memory and through registers
+    *(("soapmi_expert_product", (dtype, P, k, P, k, 0, 0, None, 1, tokens, n, k, dtype, P, n, 0, None))
+      for dtype, tokens, n, k in ((1, 1 << 21, 4096, 8), (1, 1 << 21, 4096, 9), (1, 1 << 21, 4096, 10), (1, 1 << 21, 4096, 16),
+                                  (1, 1 << 23, 1024, 8), (1, 1 << 28, 32, 16), (0, 1 << 21, 4096, 8), (0, 1 << 21, 4096, 16))),
+    ("soapmi_int8_product", (P, 16, P, P, 16, P, 1 << 21, 4096, 16, 1, P, 4096, None)),
+    # a million experts with a small matrix each
+    ("soapmi_expert_weight_gradient", (1, P, 8, P, 8, P, 1 << 20, 1 << 26, 8, 8, 1, P, 8, 64, None, 0, None)),
+])
+def test_a_product_that_some_tile_can_take_is_launched(name, arguments):
+    """The tile is chosen among those whose launch has fewer than 2^32 threads."""
+    with pytest.raises(RuntimeError, match="kernel launch failed"):
+        _native.call(name, *arguments)
