@@ -615,7 +615,19 @@ struct Unscaled {
   };
   __device__ __forceinline__ float row(int) const { return 1.0f; }
 };
-// The integer sum is exact; it is rounded to fp32 once, then scaled by the token and by the channel.
+// The integer sum is exact; it is rounded to fp32 once, then scaled by the token and by the channel.  A sum of up
+// to 2^31 times a token's scale can leave the range although the channel's brings it back: large scales of tokens
+// are applied without 2^32, which comes last.  (Nothing else can be lost on the way: an integer times a scale,
+// subnormal ones too, is no smaller than the scale.)
+struct TokenScale {
+  float scale, rest;
+  __device__ __forceinline__ explicit TokenScale(float s) {
+    const bool large = __builtin_fabsf(s) >= 0x1p96f;
+    scale = large ? s * 0x1p-32f : s;
+    rest = large ? 0x1p32f : 1.0f;
+  }
+  __device__ __forceinline__ float operator()(int sum, float channel) const { return (float)sum * scale * channel * rest; }
+};
 struct TokenChannel {
   const float* token;
   const float* channel;
@@ -628,9 +640,9 @@ struct TokenChannel {
 #pragma unroll
         for (int q = 0; q < 8; ++q) channel[i][q] = s.channel[min(c0 + 32 * i + q, cols - 1)];
     }
-    __device__ __forceinline__ float operator()(int i, int q, float token, int v) const { return (float)v * token * channel[i][q]; }
+    __device__ __forceinline__ float operator()(int i, int q, TokenScale token, int v) const { return token(v, channel[i][q]); }
   };
-  __device__ __forceinline__ float row(int r) const { return token[r]; }
+  __device__ __forceinline__ TokenScale row(int r) const { return TokenScale(token[r]); }
 };
 
 // A wavefront's results go through its share of LDS, so that it stores whole rows of its part of the tile
@@ -653,7 +665,7 @@ __device__ __forceinline__ void store_tile_as(const Result& o, const Acc (&acc)[
 #pragma unroll
     for (int jj = 0; jj < AT_ONCE; ++jj) {
       if (j0 + jj >= A) continue;
-      const float row = scale.row(min((Cfg::WR * (j0 + jj) + wr) * 16 + m, o.rows - 1));
+      const auto row = scale.row(min((Cfg::WR * (j0 + jj) + wr) * 16 + m, o.rows - 1));
 #pragma unroll
       for (int i = 0; i < Cfg::TC; i += 2) {
         Out v[8];
@@ -851,7 +863,7 @@ __device__ __forceinline__ void few_rows_tile(const RowProblem& p, const RowTile
 #pragma unroll
     for (int q = 0; q < FewTile::WAVES; ++q) v += sums[(q * A * 16 + r) * STRIDE + c];
     float out;
-    if constexpr (E::SIZE == 1) out = (float)v * p.token_scale[tile.row + r] * p.channel_scale[c0 + c];
+    if constexpr (E::SIZE == 1) out = TokenScale(p.token_scale[tile.row + r])(v, p.channel_scale[c0 + c]);
     else out = v;
     store_value(p.y, (int64_t)(tile.row + r) * p.ldy + c0 + c, p.out_type, out);
   }

@@ -779,3 +779,24 @@ def test_very_many_rows_of_short_products(device, dtype, inputs):
         wide = torch.mm(x[rows].double(), w.double().t())
         allowed = (inputs + 1) * 2.0 ** -23 * torch.mm(x[rows].double().abs(), w.double().abs().t())
         assert ((y[rows].double() - wide).abs() <= allowed + rounding(wide.abs() + allowed, dtype)).all()
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 3700])
+@pytest.mark.parametrize("token,channel", [(1e34, 1e-6), (3e38, 1e-38), (-(2.0 ** 96), 2.0 ** -96), (1e-42, 1e30), (1e-45, 3e38),
+                                           (1e30, 1e-40), (2.0 ** 127, 2.0 ** -149), (1e38, 1e20)])
+def test_int8_scales_of_any_size(device, tokens, token, channel):
+    """A token's scale alone may take the sum out of fp32's range, the channel's brings it back.  Roundings: the
+    sum to fp32, two products, and what a subnormal result loses."""
+    inputs, outputs = 64, 300
+    generator = torch.Generator(device=device).manual_seed(tokens)
+    codes = torch.randint(-127, 128, (tokens, inputs), generator=generator, device=device, dtype=torch.int8)
+    weights = torch.randint(-127, 128, (outputs, inputs), generator=generator, device=device, dtype=torch.int8)
+    codes[0], weights[0], weights[1] = 127, 127, 0  # the largest sum there is, and sums of zero
+    scales, channels = torch.full((tokens,), token, device=device), torch.full((outputs,), channel, device=device)
+    scales[-1] = 1.0
+    expected = torch.mm(codes.double(), weights.double().t()) * scales.double()[:, None] * channels.double()
+    y = products.int8_product(codes, scales, weights, channels, out_dtype=torch.float32).double()
+    finite = expected.abs() <= torch.finfo(torch.float32).max * (1 - 4 * 2.0 ** -24)
+    assert ((y - expected).abs() <= expected.abs() * 3.01 * 2.0 ** -24 + 2.0 ** -149)[finite].all()
+    beyond = expected.abs() > torch.finfo(torch.float32).max * (1 + 4 * 2.0 ** -24)
+    assert torch.equal(y[beyond], expected[beyond].sign() * float("inf"))
