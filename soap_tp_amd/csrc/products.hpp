@@ -258,8 +258,8 @@ __device__ __forceinline__ i32x4 load_bytes(const char* p, int count) {
   return v;
 }
 
-__device__ __forceinline__ float exponent_value(int code) {  // 2^(code - 127); 255: not a number
-  return __uint_as_float(code == 255 ? 0x7fc00000u : (unsigned)code << 23);
+__device__ __forceinline__ float exponent_value(int code) {  // 2^(code - 127), 0 subnormal; 255: not a number
+  return __uint_as_float(code == 255 ? 0x7fc00000u : code == 0 ? 0x00400000u : (unsigned)code << 23);
 }
 
 // One operand of a tile: BX rows (or columns), slabs of 128 bytes (KC) or 64 values (XC) of k.

@@ -800,3 +800,16 @@ def test_int8_scales_of_any_size(device, tokens, token, channel):
     assert ((y - expected).abs() <= expected.abs() * 3.01 * 2.0 ** -24 + 2.0 ** -149)[finite].all()
     beyond = expected.abs() > torch.finfo(torch.float32).max * (1 + 4 * 2.0 ** -24)
     assert torch.equal(y[beyond], expected[beyond].sign() * float("inf"))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_restoring_every_exponent(device, dtype):
+    """A checkpoint from elsewhere may hold any exponent; the values are codes * 2 ** (exponents - 127), rounded to the
+    type (products of 2^-127 are subnormal in fp32 already, and exact there)."""
+    codes = torch.arange(-127, 128, dtype=torch.int8, device=device).repeat(256, 1)
+    exponents = torch.arange(256, device=device).to(torch.uint8)[:, None].repeat(1, 2)
+    restored = products.restore_activations(products.ActivationCheckpoint(codes, exponents, dtype))
+    steps = ((torch.arange(256, device=device) - 127 + 1023) << 52).view(torch.float64)
+    expected = codes.double() * steps[:, None]
+    expected[255] = float("nan")
+    assert torch.equal(restored.nan_to_num(0.5), expected.to(dtype).nan_to_num(0.5))
