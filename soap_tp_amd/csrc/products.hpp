@@ -1068,8 +1068,12 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t 
   const bool finite = top < 0x7f800000u;
   const float largest = __uint_as_float(top);
   // Both the row and its maximum are brought to around 1 by a power of two, so that neither 127 x nor
-  // the reciprocal leaves the range.  127 x is exact for 16-bit inputs; one correction of the quotient
-  // by its remainder gives the correctly rounded one.
+  // the reciprocal leaves the range.  For 16-bit inputs 127 x is exact, one correction of the quotient by its
+  // remainder gives the correctly rounded one, and none that is not halfway between two codes is within that
+  // rounding of it.  For fp32 inputs 127 x is a + low, and where the quotient is nearly halfway the exact
+  // remainder a + low - code * b decides: it may be b / 2 at most.  Without low it is a multiple of the last
+  // place of b or a, and so is its distance to b / 2, which leaves both exact (8192 x 4096 in
+  // fp32: 34.0 us, 33.6 without it).
   int power = 0;
   const float b = frexpf(finite ? largest : 0.0f, &power);
   const float inverse = b > 0.0f ? 1.0f / b : 0.0f;
@@ -1077,12 +1081,24 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t 
   int8_t* out = codes + (int64_t)row * ldq;
   auto quantize = [&](const float (&v)[8], int c) {
     int q[8];
+    bool halfway = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float a = 127.0f * ldexpf(v[i], -power);
       float r = a * inverse;
-      r = __builtin_fmaf(__builtin_fmaf(-r, b, a), inverse, r);
+      if constexpr (sizeof(T) == 4) halfway |= __builtin_fabsf(r - __builtin_rintf(r)) > 0.4999f;  // (r is off by 2.3e-5 at most)
+      else r = __builtin_fmaf(__builtin_fmaf(-r, b, a), inverse, r);
       q[i] = finite ? (int)__builtin_rintf(r) : 0;
+    }
+    if (halfway && finite) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = ldexpf(v[i], -power), a = 127.0f * x, low = __builtin_fmaf(127.0f, x, -a);
+        const float over = __builtin_fmaf(-(float)q[i], b, a), above = over - 0.5f * b, below = over + 0.5f * b;
+        const bool odd = q[i] & 1;
+        if (above > -low || (above == -low && odd)) ++q[i];
+        else if (below < -low || (below == -low && odd)) --q[i];
+      }
     }
     store_codes(out, c * 8, cols, vec_q, q);
   };

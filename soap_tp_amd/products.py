@@ -403,7 +403,8 @@ def restore_activations(checkpoint: ActivationCheckpoint, *, out: Optional[Tenso
 
 def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
     """Codes (int8) and scales (float32, one for each row) of a matrix: scale = largest magnitude / 127,
-    code = x / scale rounded to the nearest even.  The rows are tokens, or a weight's output channels.
+    code = 127 x / largest magnitude, to the nearest, halves to even.  The rows are tokens, or a weight's
+    output channels.
     A row of zeros has scale 0; one that holds an infinity or NaN has scale NaN."""
     code = _check_values("x", x)
     index = x.get_device()

@@ -813,3 +813,19 @@ def test_restoring_every_exponent(device, dtype):
     expected = codes.double() * steps[:, None]
     expected[255] = float("nan")
     assert torch.equal(restored.nan_to_num(0.5), expected.to(dtype).nan_to_num(0.5))
+
+
+@pytest.mark.parametrize("power", [-149 + 24, -60, 0, 127])
+def test_codes_next_to_the_middle_of_two(device, power):
+    """fp32 values right at the middles between codes and one step to each side: in 64 bits 127 x is exact, and a
+    quotient of 31 by 24 bits that is not a middle is further from it than the rounding of 64 bits."""
+    generator = torch.Generator(device=device).manual_seed(5)
+    top = torch.rand(2000, 1, generator=generator, device=device) + 1
+    top[0], top[1], top[2] = 1, 1.9921875, 127 / 64  # (the latter two are 127 / 64: middles that are fp32 values)
+    middles = (torch.arange(-127, 127, device=device) + 0.5).double() * top.double() / 127
+    x = middles.float()
+    x = torch.cat([top, x, torch.nextafter(x, x + 1), torch.nextafter(x, x - 1), -top], dim=1)
+    x = torch.ldexp(x, torch.tensor(power, device=device))
+    codes, _ = products.quantize_tokens(x)
+    expected = (127 * x.double() / x[:, :1].double()).round()
+    assert torch.equal(codes.double(), expected)
