@@ -19,7 +19,9 @@ strided, sums are formed in float32 on the matrix cores.
     dw = expert_weight_gradient(dy, x, ends)                # dW_e = sum of dy[t] x[t]^T, float32
     update = soap_step(dw[e], state[e], ...)
 
-``expert_linear`` is the first of them for autograd, with the other two as its backward pass.
+``expert_linear`` is the first of them for autograd, with the other two as its backward pass.  No other call
+here is recorded by autograd: its result requires no gradient, whatever its inputs do.  A tensor given as
+``out`` counts as modified in place, and may require a gradient under ``torch.no_grad`` only.
 """
 from __future__ import annotations
 
@@ -156,6 +158,8 @@ def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, .
     _check_matrix("out", out, len(shape))
     if tuple(out.shape) != shape:
         raise ValueError(f"out has shape {tuple(out.shape)}, expected {shape}.")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out must not require a gradient: the call is not recorded by autograd.")
     if out.dtype not in dtypes:
         raise ValueError(f"out must use {' or '.join(str(d) for d in dtypes)}, got {out.dtype}.")
     if out.numel():
@@ -168,6 +172,11 @@ def _check_out(out: Tensor, shape: Tuple[int, ...], dtypes: Tuple[torch.dtype, .
             if tensor is not None and tensor.numel() and not _apart(out, tensor):
                 raise ValueError(f"out must not overlap {name}.")
     return _DTYPES[out.dtype]
+
+
+# The kernels write through addresses, which autograd does not see: a tensor that it saved for a backward pass
+# has to be known as modified.
+_modified = torch.autograd.graph.increment_version
 
 
 def _row_stride(tensor: Tensor) -> int:
@@ -206,6 +215,8 @@ def _grouped(x: Tensor, weights: Tensor, ends: Optional[Tensor], out: Optional[T
         _launch(index, "soapmi_expert_product", code, rows.data_ptr(), ldx, matrices.data_ptr(), ldw, stride_w, transposed,
                 pointer, experts, tokens, outputs, inputs, out_code, out.data_ptr(), columns if fresh else _row_stride(out),
                 1 if fresh else 0)
+        if not fresh:
+            _modified(out)
     return out
 
 
@@ -268,7 +279,8 @@ def expert_weight_gradient(
     if (index < 0 or values.get_device() != index or (saved and exponents.get_device() != index)
             or (pointer and ends.get_device() != index) or (out is not None and out.get_device() != index)):
         _refuse_devices(gradient.device, gradient=gradient, x=values, exponents=exponents, ends=ends, out=out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty(shape, dtype=out_dtype, device=gradient.device)
     if out.numel() == 0:
         return out
@@ -288,6 +300,8 @@ def expert_weight_gradient(
     _launch(index, "soapmi_expert_weight_gradient", code, gradient.data_ptr(), ldg, values.data_ptr(), ldx, pointer, experts,
             tokens, outputs, inputs, out_code, out.data_ptr(), _row_stride(out), out.stride(0) if experts > 1 else 0,
             work.data_ptr() if nbytes else 0, nbytes)
+    if not fresh:
+        _modified(out)
     return out
 
 
@@ -390,11 +404,14 @@ def restore_activations(checkpoint: ActivationCheckpoint, *, out: Optional[Tenso
     index = codes.get_device()
     if index < 0 or exponents.get_device() != index or (out is not None and out.get_device() != index):
         _refuse_devices(codes.device, codes=codes, exponents=exponents, out=out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((rows, columns), dtype=dtype, device=codes.device)
     if rows and columns:
         _launch(index, "soapmi_restore_activations", _DTYPES[dtype], codes.data_ptr(), _row_stride(codes),
                 exponents.data_ptr(), _row_stride(exponents), rows, columns, out.data_ptr(), _row_stride(out))
+        if not fresh:
+            _modified(out)
     return out
 
 
@@ -468,11 +485,14 @@ def int8_product(
             or weight_scales.get_device() != index or (out is not None and out.get_device() != index)):
         _refuse_devices(codes.device, codes=codes, scales=scales, weight_codes=weight_codes, weight_scales=weight_scales,
                         out=out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty((tokens, outputs), dtype=out_dtype, device=codes.device)
     if tokens and outputs:
         rows, ldq = _rows(codes)
         matrix, ldw = _rows(weight_codes)
         _launch(index, "soapmi_int8_product", rows.data_ptr(), ldq, scales.data_ptr(), matrix.data_ptr(), ldw,
                 weight_scales.data_ptr(), tokens, outputs, inner, out_code, out.data_ptr(), _row_stride(out))
+        if not fresh:
+            _modified(out)
     return out

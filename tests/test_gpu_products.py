@@ -829,3 +829,29 @@ def test_codes_next_to_the_middle_of_two(device, power):
     codes, _ = products.quantize_tokens(x)
     expected = (127 * x.double() / x[:, :1].double()).round()
     assert torch.equal(codes.double(), expected)
+
+
+def test_results_written_over_what_autograd_saved(device):
+    """A saved tensor that a call overwrites is found in the backward pass, as with torch's own operations."""
+    x, w = values(device, 1, 16, 32, dtype=torch.bfloat16), values(device, 2, 32, 32, dtype=torch.bfloat16)
+    saved = products.checkpoint_activations(x)
+    for rows, call in ((16, lambda out: products.expert_product(x, w, None, out=out)),
+                       (16, lambda out: products.expert_input_gradient(x, w, None, out=out)),
+                       (32, lambda out: products.expert_weight_gradient(x, w[:16], None, out=out)),
+                       (16, lambda out: products.restore_activations(saved, out=out)),
+                       (16, lambda out: products.int8_product(*products.quantize_tokens(x), *products.quantize_tokens(w), out=out))):
+        kept = torch.zeros(rows, 32, dtype=torch.bfloat16, device=device)
+        leaf = torch.ones_like(kept, requires_grad=True)
+        product = leaf * kept
+        call(kept)
+        assert kept.any()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+    held = torch.nn.Parameter(torch.zeros(16, 32, dtype=torch.bfloat16, device=device))
+    with torch.no_grad():
+        products.expert_product(x, w, None, out=held)
+    assert torch.equal(held.detach(), products.expert_product(x, w, None))
+    with torch.inference_mode():
+        out = torch.zeros(16, 32, dtype=torch.bfloat16, device=device)
+        products.expert_product(x, w, None, out=out)
+    assert torch.equal(out, held.detach())

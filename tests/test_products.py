@@ -216,3 +216,20 @@ def test_a_product_that_some_tile_can_take_is_launched(name, arguments):
     """The tile is chosen among those whose launch has fewer than 2^32 threads."""
     with pytest.raises(RuntimeError, match="kernel launch failed"):
         _native.call(name, *arguments)
+
+
+def test_out_does_not_require_a_gradient():
+    codes, scales = torch.zeros(6, 8, dtype=torch.int8), torch.zeros(6)
+
+    def calls(out):
+        return (lambda: products.expert_product(X, torch.zeros(8, 8), None, out=out),
+                lambda: products.expert_input_gradient(X, torch.zeros(8, 8), None, out=out),
+                lambda: products.expert_weight_gradient(torch.zeros(9, 6), torch.zeros(9, 8), None, out=out),
+                lambda: products.restore_activations(_saved(), out=out),
+                lambda: products.int8_product(codes, scales, torch.zeros(8, 8, dtype=torch.int8), torch.zeros(8), out=out))
+
+    for call in calls(torch.zeros(6, 8, requires_grad=True)):
+        with pytest.raises(ValueError, match="out must not require a gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="requires cuda buffers"):
+            call()
