@@ -309,14 +309,13 @@ class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weights, ends, checkpoint):
         y = expert_product(x, weights, ends)
-        kept = x
-        if ctx.needs_input_grad[1] and checkpoint:
-            kept = checkpoint_activations(x)
-        ctx.dtype = x.dtype
-        if isinstance(kept, ActivationCheckpoint):
-            ctx.save_for_backward(weights, ends, kept.codes, kept.exponents)
-        else:
-            ctx.save_for_backward(weights, ends, x if ctx.needs_input_grad[1] else None, None)
+        # each operand is kept for the other's gradient
+        needed = weights if ctx.needs_input_grad[0] else None
+        kept, exponents = (x if ctx.needs_input_grad[1] else None), None
+        if kept is not None and checkpoint:
+            kept, exponents, _ = checkpoint_activations(x)
+        ctx.dtype, ctx.out_dtype = x.dtype, weights.dtype
+        ctx.save_for_backward(needed, ends, kept, exponents)
         return y
 
     @staticmethod
@@ -328,7 +327,7 @@ class _ExpertLinear(torch.autograd.Function):
             dx = expert_input_gradient(gradient, weights, ends)
         if ctx.needs_input_grad[1]:
             x = kept if exponents is None else ActivationCheckpoint(kept, exponents, ctx.dtype)
-            dw = expert_weight_gradient(gradient, x, ends, out_dtype=weights.dtype)
+            dw = expert_weight_gradient(gradient, x, ends, out_dtype=ctx.out_dtype)
         return dx, dw, None, None
 
 

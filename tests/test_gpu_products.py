@@ -855,3 +855,25 @@ def test_results_written_over_what_autograd_saved(device):
         out = torch.zeros(16, 32, dtype=torch.bfloat16, device=device)
         products.expert_product(x, w, None, out=out)
     assert torch.equal(out, held.detach())
+
+
+def test_expert_linear_keeps_what_its_gradients_need(device):
+    """An operand may change before the backward pass if only its own gradient is asked for."""
+    x, weights = values(device, 1, 30, 16, dtype=torch.bfloat16), values(device, 2, 2, 8, 16, dtype=torch.bfloat16)
+    dy, ends = values(device, 3, 30, 8, dtype=torch.bfloat16), torch.tensor([10, 30], device=device)
+    held = weights.clone().requires_grad_()
+    y = products.expert_linear(x, held, ends)
+    with torch.no_grad():
+        held.mul_(2)  # (an optimizer's step)
+    y.backward(dy)
+    assert torch.equal(held.grad, products.expert_weight_gradient(dy, x, ends, out_dtype=torch.bfloat16))
+    rows, frozen = x.clone().requires_grad_(), weights.clone()
+    y = products.expert_linear(rows, frozen, ends)
+    with torch.no_grad():
+        rows.mul_(2)
+    y.backward(dy)
+    assert torch.equal(rows.grad, products.expert_input_gradient(dy, weights, ends))
+    y = products.expert_linear(rows, frozen, ends)
+    frozen.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
