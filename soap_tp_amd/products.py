@@ -307,14 +307,16 @@ def expert_weight_gradient(
 
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weights, ends, checkpoint):
+    def forward(ctx, x, weights, ends, checkpoint, mixed):
+        ctx.dtype, ctx.out_dtype = x.dtype, weights.dtype
+        if mixed:
+            weights = weights.to(x.dtype)
         y = expert_product(x, weights, ends)
         # each operand is kept for the other's gradient
         needed = weights if ctx.needs_input_grad[0] else None
         kept, exponents = (x if ctx.needs_input_grad[1] else None), None
         if kept is not None and checkpoint:
             kept, exponents, _ = checkpoint_activations(x)
-        ctx.dtype, ctx.out_dtype = x.dtype, weights.dtype
         ctx.save_for_backward(needed, ends, kept, exponents)
         return y
 
@@ -328,7 +330,7 @@ class _ExpertLinear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             x = kept if exponents is None else ActivationCheckpoint(kept, exponents, ctx.dtype)
             dw = expert_weight_gradient(gradient, x, ends, out_dtype=ctx.out_dtype)
-        return dx, dw, None, None
+        return dx, dw, None, None, None
 
 
 def expert_linear(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, checkpoint: bool = False) -> Tensor:
@@ -339,10 +341,22 @@ def expert_linear(x: Tensor, weights: Tensor, ends: Optional[Tensor], *, checkpo
     instead of in its own type; the weights' gradient is then that of the restored input, ``x``'s
     gradient and the result are unchanged.
 
+    Under ``torch.autocast`` the product and the gradients are formed in autocast's type.  Weights kept in
+    float32 then get their gradient in float32, as the sums are: it is not rounded on the way.
+
     To capture it with its backward pass into a graph, capture both together and let no earlier autograd
     graph of the same leaves live: torch accumulates a leaf's gradient on the stream of the first graph that
     holds the leaf, and a capture cannot wait for that stream."""
-    return _ExpertLinear.apply(x, weights, ends, checkpoint)
+    mixed = False
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        _check_values("x", x)
+        _check_values("weights", weights, 2 if ends is None else 3)
+        x = x.to(dtype)
+        mixed = weights.dtype == torch.float32 != dtype
+        if not mixed and weights.dtype != dtype:
+            weights = weights.to(dtype)
+    return _ExpertLinear.apply(x, weights, ends, checkpoint, mixed)
 
 
 # ---- activation checkpoints ----------------------------------------------------------------

@@ -877,3 +877,55 @@ def test_expert_linear_keeps_what_its_gradients_need(device):
     frozen.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("x_dtype,weights_dtype", [(torch.float32, torch.float32), (None, torch.float32), (torch.float32, None),
+                                                   (torch.bfloat16, torch.float16), (None, None)], ids=str)
+def test_expert_linear_under_autocast(device, dtype, x_dtype, weights_dtype, checkpoint):
+    """In autocast's type, whatever the operands' (None: that one); float32 weights get the sums' own float32."""
+    x = values(device, 1, 90, 136, dtype=x_dtype or dtype).requires_grad_()
+    weights = values(device, 2, 3, 40, 136, dtype=weights_dtype or dtype).requires_grad_()
+    dy, ends = values(device, 3, 90, 40, dtype=dtype), torch.tensor([30, 30, 85], device=device)
+    with torch.autocast("cuda", dtype=dtype):
+        y = products.expert_linear(x, weights, ends, checkpoint=checkpoint)
+    y.backward(dy)
+    rows, matrices = x.detach().to(dtype), weights.detach().to(dtype)
+    kept = products.checkpoint_activations(rows) if checkpoint else rows
+    assert y.dtype == dtype and torch.equal(y.detach(), products.expert_product(rows, matrices, ends))
+    assert torch.equal(x.grad, products.expert_input_gradient(dy, matrices, ends).to(x.dtype))
+    sums = products.expert_weight_gradient(dy, kept, ends)
+    assert torch.equal(weights.grad, sums if weights.dtype == torch.float32 else sums.to(dtype).to(weights.dtype))
+    with torch.autocast("cuda", dtype=dtype), pytest.raises(ValueError, match="x must use float32, bfloat16 or float16"):
+        products.expert_linear(x.double(), weights, ends)
+
+
+def test_experts_trained_by_the_optimizer(device):
+    """Experts' matrices as parameters of their own, in float32 under autocast: the optimizer takes each one's
+    gradient as it is, and steps as soap_step does."""
+    from soap_tp_amd import SOAP, soap_step
+
+    experts, outputs, inputs, tokens = 3, 24, 32, 90
+    ends = torch.tensor([40, 64, 85], device=device)
+    weights = [torch.nn.Parameter(values(device, e, outputs, inputs, dtype=torch.float32)) for e in range(experts)]
+    mirrors, states = [w.detach().clone() for w in weights], [{} for _ in weights]
+    optimizer = SOAP(weights, lr=0.01, betas=(0.9, 0.95), eps=1e-6, weight_decay=0.0, precondition_frequency=100)
+    for iteration in range(4):
+        x = values(device, 100 + iteration, tokens, inputs, dtype=torch.bfloat16)
+        dy = values(device, 200 + iteration, tokens, outputs, dtype=torch.bfloat16)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            y = products.expert_linear(x, torch.stack(weights), ends)
+        y.backward(dy)
+        dw = products.expert_weight_gradient(dy, x, ends)
+        for e, w in enumerate(weights):
+            assert torch.equal(w.grad, dw[e])
+            update = soap_step(dw[e], states[e], global_shape=(outputs, inputs), shard_dim=1, block_size=128,
+                               process_grid_shape=(1, 1), preconditioner_beta=0.95, beta1=0.9, beta2=0.95, eps=1e-6,
+                               basis_refresh_interval=100)
+            if iteration:
+                mirrors[e] -= 0.01 * update
+        optimizer.step()
+        optimizer.zero_grad()
+        for w, mirror in zip(weights, mirrors):
+            assert (w.detach() - mirror).norm() <= 1e-5 * mirror.norm()
