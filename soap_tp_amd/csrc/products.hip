@@ -26,7 +26,10 @@ static __global__ __launch_bounds__(256) void join_parts_kernel(SumProblem p) {
   for (int part = 1; part < p.parts; ++part) sum += p.partials[part * all + at];
   const int64_t e = at / matrix, in = at - e * matrix;
   const int64_t r = in / p.cols, c = in - r * p.cols;
-  store_value(p.d, e * p.stride_d + r * p.ldd + c, p.out_type, sum);
+  const int64_t to = e * p.stride_d + r * p.ldd + c;
+  if (p.out_type == kFloat32) static_cast<float*>(p.d)[to] = sum;
+  else if (p.out_type == kBFloat16) static_cast<__bf16*>(p.d)[to] = (__bf16)sum;
+  else static_cast<_Float16*>(p.d)[to] = (_Float16)sum;
 }
 
 int launch_join(hipStream_t stream, const SumProblem& p) {

@@ -35,8 +35,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 enum : int { kFloat32 = 0, kBFloat16 = 1, kFloat16 = 2 };  // SOAPMI_FLOAT32 ...
 
+// SIZE: bytes of an operand's value.  Value: the type that a result may have beside fp32 (8-bit products: any).
 struct ElemBF16 {
   static constexpr int SIZE = 2;
+  using Value = __bf16;
   using Acc = f32x4;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -44,6 +46,7 @@ struct ElemBF16 {
 };
 struct ElemF16 {
   static constexpr int SIZE = 2;
+  using Value = _Float16;
   using Acc = f32x4;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -51,6 +54,7 @@ struct ElemF16 {
 };
 struct ElemF32 {
   static constexpr int SIZE = 4;
+  using Value = float;
   using Acc = f32x4;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {  // four values of k, one after the other
     const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
@@ -61,6 +65,7 @@ struct ElemF32 {
 };
 struct ElemI8 {
   static constexpr int SIZE = 1;
+  using Value = void;
   using Acc = i32x4;
   static __device__ __forceinline__ Acc mma(i32x4 a, i32x4 b, Acc c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
@@ -591,10 +596,19 @@ struct Result {
   int type;        // kFloat32, kBFloat16, kFloat16
 };
 
-__device__ __forceinline__ void store_value(void* base, int64_t at, int type, float v) {
-  if (type == kFloat32) static_cast<float*>(base)[at] = v;
-  else if (type == kBFloat16) static_cast<__bf16*>(base)[at] = (__bf16)v;
-  else static_cast<_Float16*>(base)[at] = (_Float16)v;
+// f(a value of the type that results of E's products have).  Only those that the entry points let through.
+template <class E, class F>
+__device__ __forceinline__ void with_result_type(int type, F f) {
+  if constexpr (std::is_void_v<typename E::Value>) {
+    if (type == kFloat32) f(float{});
+    else if (type == kBFloat16) f(__bf16{});
+    else f(_Float16{});
+  } else if constexpr (std::is_same_v<typename E::Value, float>) {
+    f(float{});
+  } else {
+    if (type == kFloat32) f(float{});
+    else f(typename E::Value{});
+  }
 }
 
 // Eight consecutive values, at any address (memory takes 16 bytes anywhere).
@@ -704,12 +718,11 @@ __device__ __forceinline__ void store_tile_as(const Result& o, const Acc (&acc)[
   }
 }
 
-template <class Cfg, int A, class Acc, class Scale>
-__device__ __forceinline__ void store_tile(const Result& o, const Acc (&acc)[A][Cfg::TC], const Scale& scale, char* lds) {
+template <class E, class Cfg, int A, class Scale>
+__device__ __forceinline__ void store_tile(const Result& o, const typename E::Acc (&acc)[A][Cfg::TC], const Scale& scale,
+                                           char* lds) {
   barrier();  // every wavefront is done with the operands
-  if (o.type == kFloat32) store_tile_as<Cfg, float, A>(o, acc, scale, lds);
-  else if (o.type == kBFloat16) store_tile_as<Cfg, __bf16, A>(o, acc, scale, lds);
-  else store_tile_as<Cfg, _Float16, A>(o, acc, scale, lds);
+  with_result_type<E>(o.type, [&](auto value) { store_tile_as<Cfg, decltype(value), A>(o, acc, scale, lds); });
 }
 
 // ---- kernels -------------------------------------------------------------------------------
@@ -750,9 +763,9 @@ __device__ __forceinline__ void row_tile(const RowProblem& p, const RowTile& til
   o.cols = c.valid;
   o.type = p.out_type;
   if constexpr (E::SIZE == 1)
-    store_tile<Cfg, A>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0}, lds);
+    store_tile<E, Cfg, A>(o, acc, TokenChannel{p.token_scale + tile.row, p.channel_scale + c0}, lds);
   else
-    store_tile<Cfg, A>(o, acc, Unscaled{}, lds);
+    store_tile<E, Cfg, A>(o, acc, Unscaled{}, lds);
 }
 
 template <class E, Layout LC, Source S, class Cfg, int A>
@@ -865,7 +878,8 @@ __device__ __forceinline__ void few_rows_tile(const RowProblem& p, const RowTile
     float out;
     if constexpr (E::SIZE == 1) out = TokenScale(p.token_scale[tile.row + r])(v, p.channel_scale[c0 + c]);
     else out = v;
-    store_value(p.y, (int64_t)(tile.row + r) * p.ldy + c0 + c, p.out_type, out);
+    const int64_t to = (int64_t)(tile.row + r) * p.ldy + c0 + c;
+    with_result_type<E>(p.out_type, [&](auto value) { static_cast<decltype(value)*>(p.y)[to] = (decltype(value))out; });
   }
 }
 
@@ -983,7 +997,7 @@ __global__ __launch_bounds__(Cfg::NT) void sum_product_kernel(SumProblem p) {
   Result o = sum_result(p, tile, r0, c0);
   o.rows = r.valid;
   o.cols = c.valid;
-  store_tile<Cfg, Cfg::TR>(o, acc, Unscaled{}, lds);
+  store_tile<E, Cfg, Cfg::TR>(o, acc, Unscaled{}, lds);
 }
 
 // ---- 8-bit codes ---------------------------------------------------------------------------
