@@ -929,3 +929,76 @@ def test_experts_trained_by_the_optimizer(device):
         optimizer.zero_grad()
         for w, mirror in zip(weights, mirrors):
             assert (w.detach() - mirror).norm() <= 1e-5 * mirror.norm()
+
+
+# ---- sums are held in 32 bits --------------------------------------------------------------
+#
+# The bound above grows with the terms, as a worst case does, and over thousands of them it would let sums in 16
+# bits pass.  Whole numbers leave no room: every partial sum below 2^24 is exact in fp32, in any order, and odd
+# ones above 2^11 are in neither of the 16-bit types.  For random values the norms are compared: a sum of n terms
+# is rounded n times at most, each time by a step (2^-23) of a partial sum, which is sqrt(i / n) of the whole one
+# after i terms; independent of each other, such errors have a root mean square below 2^-23 sqrt(n / 2) of the
+# result's, and 8 times that is far below the 2^-9 sqrt(n / 2) and more of a sum kept in bf16 or the 2^-12 sqrt(n / 2)
+# of one in fp16, even if it is rounded only every 64 rows.
+
+
+def whole_numbers(device, seed, *shape, dtype):
+    generator = torch.Generator(device=device).manual_seed(seed)
+    return torch.randint(0, 9, shape, generator=generator, device=device).to(dtype)
+
+
+LONG = [(6000, 1, 72, 80), (5000, 2, 130, 257), (4100, 3, 264, 3584), (3584, 1, 512, 4100), (40, 2, 16, 6000), (40, 2, 6000, 16)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sums_of_whole_numbers_are_exact(device, dtype, shape):
+    tokens, experts, outputs, inputs = shape
+    x, weights = whole_numbers(device, 1, tokens, inputs, dtype=dtype), whole_numbers(device, 2, experts, outputs, inputs, dtype=dtype)
+    dy = whole_numbers(device, 3, tokens, outputs, dtype=dtype)
+    spans, ends = split(tokens, experts, device, seed=sum(shape))
+    wide = [torch.empty(tokens, n, device=device) for n in (outputs, inputs)]
+    products.expert_product(x, weights, ends, out=wide[0])
+    products.expert_input_gradient(dy, weights, ends, out=wide[1])
+    assert torch.equal(wide[0].double(), forward_exact(x, weights, spans))
+    assert torch.equal(wide[1].double(), forward_exact(dy, weights.transpose(1, 2), spans))
+    expected = sums_exact(dy, x, spans)
+    assert expected.max() < 2 ** 24 and (tokens < 1000 or (expected.max() > 2 ** 13 and (expected % 2 == 1).any()))
+    assert torch.equal(products.expert_weight_gradient(dy, x, ends).double(), expected)
+    assert torch.equal(products.expert_weight_gradient(dy, products.checkpoint_activations(x), ends).double(), expected)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sums_in_norm(device, dtype, shape):
+    tokens, experts, outputs, inputs = shape
+    x, weights = values(device, 1, tokens, inputs, dtype=dtype), values(device, 2, experts, outputs, inputs, dtype=dtype)
+    dy = values(device, 3, tokens, outputs, dtype=dtype)
+    spans, ends = split(tokens, experts, device, seed=sum(shape))
+
+    def assert_near(actual, expected, terms):
+        off, size = (actual.double() - expected).norm().item(), expected.norm().item()
+        assert off <= 8 * 2.0 ** -23 * max(1.0, terms / 2) ** 0.5 * size, (off / size, terms)
+
+    y, dx = torch.empty(tokens, outputs, device=device), torch.empty(tokens, inputs, device=device)
+    products.expert_product(x, weights, ends, out=y)
+    products.expert_input_gradient(dy, weights, ends, out=dx)
+    assert_near(y, forward_exact(x, weights, spans), inputs)
+    assert_near(dx, forward_exact(dy, weights.transpose(1, 2), spans), outputs)
+    dw, expected = products.expert_weight_gradient(dy, x, ends), sums_exact(dy, x, spans)
+    for e, (first, last) in enumerate(spans):  # with each expert's own number of terms, element by element too
+        assert_near(dw[e], expected[e], last - first)
+        magnitudes = torch.mm(dy[first:last].double().abs().t(), x[first:last].double().abs())
+        assert_product(dw[e], expected[e], magnitudes, last - first)
+
+
+def test_the_norms_would_show_sums_in_16_bits(device):
+    """On the CPU: the same sizes with an accumulator that is rounded every 64 rows."""
+    for tokens in (6000, 4100):
+        x, dy = (values(torch.device("cpu"), seed, tokens, 64, dtype=torch.float32).bfloat16().float() for seed in (1, 2))
+        expected = torch.mm(dy.double().t(), x.double())
+        for kept in HALF:
+            total = torch.zeros(64, 64)
+            for first in range(0, tokens, 64):
+                total = (total + torch.mm(dy[first:first + 64].t(), x[first:first + 64])).to(kept).float()
+            assert (total.double() - expected).norm() > 8 * 2.0 ** -23 * (tokens / 2) ** 0.5 * expected.norm()
