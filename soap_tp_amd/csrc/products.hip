@@ -220,7 +220,8 @@ int soapmi_expert_weight_gradient(int dtype, const void* gradient, int64_t ldg, 
 }
 
 size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t tokens, int64_t n, int64_t k) {
-  return experts > 0 && tokens > 0 && n > 0 && k > 0 ? sum_partials_bytes(experts, tokens, n, k) : 0;
+  const bool fits = experts < kSizeLimit && tokens < kSizeLimit && n < kSizeLimit && k < kSizeLimit;  // others are refused
+  return fits && experts > 0 && tokens > 0 && n > 0 && k > 0 ? sum_partials_bytes(experts, tokens, n, k) : 0;
 }
 
 int soapmi_checkpoint_activations(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes,

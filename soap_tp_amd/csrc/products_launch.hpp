@@ -133,9 +133,9 @@ int row_products(hipStream_t stream, const RowProblem& p, bool direct) {
 // compute units and the sums are long: as many as fill them, of 8 slabs of 64 rows at least.  65536 rows of
 // 512 x 512, bf16: 530 us whole, 78 us in parts; 16384 rows of 1024 x 1024: 108 and 58.
 inline int sum_parts(int64_t experts, int64_t tokens, int64_t rows, int64_t cols) {
-  const int64_t tiles = experts * ceil_div64(rows, 128) * ceil_div64(cols, 128);
-  if (experts <= 0 || tiles <= 0 || tiles > 128) return 1;
-  return (int)std::max<int64_t>(1, std::min(256 / tiles, tokens / experts / 512));
+  const int64_t tiles = ceil_div64(rows, 128) * ceil_div64(cols, 128);  // of a matrix
+  if (experts <= 0 || tiles <= 0 || tiles > 128 / experts) return 1;
+  return (int)std::max<int64_t>(1, std::min(256 / (experts * tiles), tokens / experts / 512));
 }
 inline size_t sum_partials_bytes(int64_t experts, int64_t tokens, int64_t rows, int64_t cols) {
   const int parts = sum_parts(experts, tokens, rows, cols);

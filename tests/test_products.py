@@ -233,3 +233,17 @@ def test_out_does_not_require_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="requires cuda buffers"):
             call()
+
+
+@pytest.mark.parametrize("experts,tokens,n,k", [
+    (1, 1 << 20, 318550919442291584, 632734031689253760),  # as many tiles as 1 in 64 bits
+    (1, 1 << 40, 64, 64), ((1 << 30) - 1, (1 << 30) - 1, (1 << 30) - 1, (1 << 30) - 1), (64, 1 << 20, 256, 256), (129, 1 << 20, 8, 8),
+    (0, 1 << 20, 8, 8), (1, 1 << 20, -8, 8), (1, 1023, 8, 8)])
+def test_no_workspace_where_sums_stay_whole(experts, tokens, n, k):
+    assert _native.library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, n, k) == 0
+
+
+@pytest.mark.parametrize("experts,tokens,n,k,parts", [(1, 1 << 20, 8, 8, 256), (128, 1 << 20, 8, 8, 2), (2, 2048, 300, 500, 2),
+                                                      (1, 6000, 72, 80, 11), (1, 1024, 8, 8, 2)])
+def test_workspace_of_cut_sums(experts, tokens, n, k, parts):
+    assert _native.library().soapmi_expert_weight_gradient_workspace_bytes(experts, tokens, n, k) == parts * experts * n * k * 4
