@@ -201,7 +201,10 @@ int soapmi_col_major_to_row_major_f32(const float* in, int64_t ldi, float* out, 
  * expert e's starts e * stride elements after the first.  `dtype` and `out_dtype` are one of the
  * SOAPMI_FLOAT32, SOAPMI_BFLOAT16, SOAPMI_FLOAT16; sums are formed in fp32 on the matrix cores (8-bit
  * codes: exactly, in 32-bit integers) and rounded once.  Results do not depend on scheduling.
- * tokens, n, k < 2^30.  Buffers of one call must not overlap.  Where an operand's rows start at multiples
+ * tokens, n, k < 2^30, and a launch has fewer than 2^32 threads: a product may have fewer than 2^23 tiles of
+ * 128 x 128 results or 2^24 of 32 x 128 (an expert's last tile may be cut short), a matrix that is
+ * checkpointed or restored fewer than 2^35 values, one that is quantised fewer than 2^24 rows, 2^26 of up to
+ * 1024 columns.  What does not fit is refused (SOAPMI_INVALID_ARGUMENT).  Buffers of one call must not overlap.  Where an operand's rows start at multiples
  * of 16 bytes, they are read in whole pieces of 16 bytes: what stands behind a row's last value in its
  * last piece is read, and does not matter. */
 #define SOAPMI_FLOAT32 0
@@ -233,7 +236,8 @@ size_t soapmi_expert_weight_gradient_workspace_bytes(int64_t experts, int64_t to
  * -127..127, exponent = log2(step) + 127.  A value is restored as code * step, off by at most half a step
  * (one step above 127.5 steps).  Columns that hold an infinity or NaN get exponent 255 and are restored as NaN.
  * A step is a power of two, so that code * step is exact in the type it came from: a weight gradient's
- * products of restored values are those of the codes. */
+ * products of restored values are those of the codes (there is no call that takes the codes: restore the matrix
+ * first).  Restoring takes any exponent, 0 as 2^-127, and rounds code * 2^(exponent-127) to the type. */
 int soapmi_checkpoint_activations(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* codes,
                                   int64_t ldq, uint8_t* exponents, int64_t lde, void* stream);
 int soapmi_restore_activations(int dtype, const int8_t* codes, int64_t ldq, const uint8_t* exponents, int64_t lde,
@@ -246,7 +250,8 @@ int soapmi_quantize_rows(int dtype, const void* x, int64_t ldx, int64_t rows, in
                          float* scales, void* stream);
 
 /* y[t, j] = scales[t] * w_scales[j] * sum over i of codes[t, i] * w_codes[j, i]; codes: tokens x k, w_codes:
- * n x k, k <= 131071 (the integer sum stays inside 32 bits), y: tokens x n. */
+ * n x k, k <= 131071 (the integer sum stays inside 32 bits), y: tokens x n.  The sum is rounded to fp32, multiplied by
+ * one scale, then by the other; no product on the way leaves fp32's range unless the result does. */
 int soapmi_int8_product(const int8_t* codes, int64_t ldq, const float* scales, const int8_t* w_codes, int64_t ldw,
                         const float* w_scales, int64_t tokens, int64_t n, int64_t k, int out_dtype, void* y, int64_t ldy,
                         void* stream);

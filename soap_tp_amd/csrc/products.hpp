@@ -430,8 +430,8 @@ struct ProductTile {
 // loads of a whole slab in a row would keep it from issuing anything else for as long as they take
 // (8192^3 on 256 x 256 tiles: 850 us with the loads at the slab's start, 790 with them dealt out).
 //
-// What bounds it there: the matrix cores are busy for 72 % of the time (forward; the others 76-78 %) at a
-// clock that power holds at 1.5 - 1.9 GHz; without loads the same code takes 650 us, on zero operands 650-700.
+// What bounds it there: the matrix cores are busy for 72 - 77 % of the time at a clock that power holds at 1.8 -
+// 1.9 GHz of 2.4 (forward 760 - 790 us); without loads the same code takes 650 us, on zero operands 650-700.
 template <class E, Layout LR, Layout LC, Source S, class Cfg, int A = Cfg::TR>
 struct TileProduct {
   static constexpr bool DIRECT = S == Direct;
@@ -792,7 +792,7 @@ __global__ __launch_bounds__(Cfg::NT) void row_product_kernel(RowProblem p) {
 // workgroup has 32 outputs and up to 32 rows of one expert; its eight wavefronts take every eighth 128
 // bytes of k, straight from memory to the matrix instruction's registers: no wavefront waits for
 // another one before the end, so all of a compute unit's loads are in flight at once.  The eight sums
-// meet in LDS and are added in order.  One row, 11008 x 4096 in 8 bits: 11.8 us = 3.8 TB/s; one row, 4096 x
+// meet in LDS and are added in order.  One row, 11008 x 4096 in 8 bits: 12.2 us = 3.7 TB/s; one row, 4096 x
 // 4096 bf16: 13.1 us against 19.7 on 32 x 128 tiles.
 struct FewTile {
   static constexpr int BR = 32, BC = 32, WAVES = 8, NT = 64 * WAVES;
@@ -1042,7 +1042,7 @@ constexpr int kRowRegisters = 4;  // chunks of eight values that a thread keeps 
 // codes = round(127 x / top), scale = top / 127, with top the largest magnitude of the row.  A row of
 // zeros has scale 0; a row that holds an infinity or NaN has scale NaN and codes 0, so that everything
 // it stands for is NaN.  TPR threads take a row and keep up to 32 values each, so that a row of up to 8192
-// is read once.  Bound by memory: 8192 x 4096 bf16 in 20 us = 5.1 TB/s.
+// is read once.  Bound by memory: 8192 x 4096 bf16 in 25.5 us = 4.0 TB/s, in 20 us if the last-level cache has it.
 template <class T, int TPR>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* x, int64_t ldx, int rows, int cols, int vec_x,
                                                             int8_t* codes, int64_t ldq, int vec_q, float* scales) {
@@ -1134,9 +1134,9 @@ constexpr int kCheckpointBlock = 128;  // columns that share an exponent
 // step is 2^(p-7) (at least 2^-126; 2^-24, the smallest fp16 value, for fp16) and the codes are
 // round(x / step) held to -127..127; the exponent is stored with 127 added, 255 marks a block that holds
 // an infinity or NaN.  The step is a power of two because it stands inside the weight gradient's sum:
-// code * step is then exact in 16 bits, and so is
-// its product with a 16-bit gradient in fp32.  Sixteen lanes take a block.  Bound by memory: 8192 x 4096
-// bf16 in 21 us = 4.8 TB/s (restored in 19.5 us).
+// code * step is then exact in 16 bits, and so is its product with a 16-bit gradient in fp32.  Sixteen lanes
+// take a block.  Bound by memory: 8192 x 4096
+// bf16 in 24 us = 4.2 TB/s (21.5 us if the last-level cache has it; restored in 18.7 us = 5.4 TB/s).
 template <class T>
 __global__ __launch_bounds__(256) void checkpoint_kernel(const T* x, int64_t ldx, int64_t rows, int cols, int blocks,
                                                          int vec_x, int8_t* codes, int64_t ldq, int vec_q,

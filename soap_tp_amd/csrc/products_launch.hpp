@@ -105,7 +105,13 @@ double few_rows_time(const RowProblem& p) {
 // chip idle for long (input gradient, low / small / mid: 500 rows, 2048 x 512: 47.6 / 34.0 / 126; 100 rows, 1024 x
 // 1024: 26.4 / 19.1 / 65.9; 4 experts of 1024 x 1100, 1000 rows: 43.3 / 37.0 / 66.7; 1024 rows, 1024 x 1024:
 // 29.0 / 28.9 / 66.7; forward, 2048^3: 147 / 167 / 128).  At 16 bits, where the slabs' latency bounds small
-// products, it is no clear gain (low / small: 1024 rows, 1024 x 1024: 9.9 / 10.4; 256 rows: 9.3 / 8.4).
+// products, it is no clear gain (low / small: 1024 rows, 1024 x 1024: 9.9 / 10.4; 256 rows: 9.3 / 8.4).  Forward in
+// fp32, few / low / small / mid / wide: 4 experts of 1024 x 1024 with 8 rows each: 9.6 / 25 / 17 / 37 / 65; 1000 rows,
+// 4 x 1024 x 1100: 36 / 29 / 32 / 71 / 259 (taken: low, 28); 4096^3: 1845 / 1097 / 1127 / 968 / 927.
+// Staged tiles are chosen by the direct ones' figures, although a slab takes two or three times as long.  bf16, few /
+// low / mid: forward, 1500 rows of 24 experts, 1111 x 777: 56 / 22.4 / 16.9 (taken: mid); 2048 rows, 2047 x 2047: 402 /
+// 70 / 35 (mid); 1024 rows, 1023 x 1023: 57 / 19.2 / 21.5 (low); 300 rows: 30.2 / 18.3 / 20.5 (few: not the best);
+// input gradient of 1024 rows, 1023 x 1023: - / 50.4 / 37.8 (low: not the best).
 template <class E, Layout LC, Source S>
 int launch_rows(hipStream_t stream, const RowProblem& p) {
   constexpr bool has_small = S == Direct && E::SIZE == 4;
@@ -131,7 +137,9 @@ int row_products(hipStream_t stream, const RowProblem& p, bool direct) {
 
 // Parts that the experts' rows are cut into when the tiles (of 128 x 128) fill less than half of the 256
 // compute units and the sums are long: as many as fill them, of 8 slabs of 64 rows at least.  65536 rows of
-// 512 x 512, bf16: 530 us whole, 78 us in parts; 16384 rows of 1024 x 1024: 108 and 58.
+// 512 x 512, bf16: 530 us whole, 78 us in parts; 16384 rows of 1024 x 1024: 108 and 58.  The rows are only known on
+// the device and taken as shared evenly: one expert with nearly all of them gets no more parts than the others (8
+// experts of 512 x 512, 65536 rows: 79 us shared evenly, 280 with all but 448 rows at one).
 inline int sum_parts(int64_t experts, int64_t tokens, int64_t rows, int64_t cols) {
   const int64_t tiles = ceil_div64(rows, 128) * ceil_div64(cols, 128);  // of a matrix
   if (experts <= 0 || tiles <= 0 || tiles > 128 / experts) return 1;

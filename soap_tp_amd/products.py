@@ -12,7 +12,8 @@ expert may have no row, and the buffer may have rows behind the last expert's.  
 device, so nothing here depends on their values on the host and calls can be captured into a graph.
 Weights are (outputs, inputs) matrices, ``(experts, outputs, inputs)`` with experts; a dense layer
 passes ``ends=None`` and two-dimensional weights.  Inputs are bfloat16, float16 or float32, rows may be
-strided, sums are formed in float32 on the matrix cores.
+strided, sums are formed in float32 on the matrix cores.  An input whose rows are not contiguous (a transposed
+matrix or stack of weights) is copied first, on every call.
 
     y  = expert_product(x, weights, ends)                   # y[t] = W_e x[t]
     dx = expert_input_gradient(dy, weights, ends)           # dx[t] = W_e^T dy[t]
@@ -248,8 +249,9 @@ def expert_weight_gradient(
     without ``ends``; zeros for an expert without rows.
 
     ``gradient`` is (tokens, outputs); ``x`` (tokens, inputs) of the same type, or the checkpoint that
-    was made from it.  The result is float32, the type ``soap_step`` takes, or ``out_dtype`` (the
-    gradient's own type); ``out`` receives it instead of a new tensor."""
+    was made from it, which is restored for the time of the call (in memory of its own).  The result is
+    float32, the type ``soap_step`` takes, or ``out_dtype`` (the gradient's own type); ``out`` receives it
+    instead of a new tensor, in its own type."""
     code = _check_values("gradient", gradient)
     saved = isinstance(x, ActivationCheckpoint)
     if saved:
@@ -392,7 +394,9 @@ def _code_matrix(rows: int, columns: int, device) -> Tensor:
 def checkpoint_activations(x: Tensor) -> ActivationCheckpoint:
     """Keep a matrix in 8 bits, with a power-of-two step for each row and 128 columns: half the memory
     of 16-bit activations.  A value is restored to within half a step (within a step above 127.5
-    steps), a step being at most 1/64 of the largest magnitude of its 128 columns."""
+    steps), a step being at most 1/64 of the largest magnitude of its 128 columns, or 2^-126 (float16:
+    2^-24, its smallest value) where that is more.  128 columns that hold an infinity or NaN are restored
+    as NaN."""
     code = _check_values("x", x)
     index = x.get_device()
     if index < 0:
