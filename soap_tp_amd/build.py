@@ -88,7 +88,8 @@ def unsettled_loads(listing: str) -> List[str]:
         falls_in = [] if code[at][2] or code[at - 1][0] in ("s_branch", "s_endpgm", "s_setpc_b64") else [at - 1]
         for source in falls_in + before.get(at, []):
             name, operands, _ = code[source]
-            if name.startswith("v_") and _scalar_registers(",".join(operands.split(",")[:2 if "_co_" in name else 1])) & read:
+            results = 2 if re.search("_co_|div_scale|mad_[iu]64", name) else 1  # (the second is a carry or a flag)
+            if name.startswith("v_") and _scalar_registers(",".join(operands.split(",")[:results])) & read:
                 return True
             left = states - 1 - (int(operands) if name == "s_nop" else 0)
             if left > 0 and written_near(source, left, read):
@@ -102,7 +103,10 @@ def unsettled_loads(listing: str) -> List[str]:
 def check_loads(library: Path) -> int:
     """Raise if a kernel of the library has an unsettled load, or has loads to LDS and spills registers (a
     spilled scalar register comes back through a vector instruction).  Returns how many such loads there are."""
-    tools = Path(os.path.realpath(hipcc_path())).parent.parent / "llvm" / "bin"
+    places = (Path(os.path.realpath(hipcc_path())).parent.parent / "llvm" / "bin", Path("/opt/rocm/llvm/bin"))
+    tools = next((place for place in places if (place / "llvm-objdump").exists()), None)
+    if tools is None:
+        raise RuntimeError("llvm-objdump was not found; the loads to LDS cannot be checked.")
     loads = 0
     with tempfile.TemporaryDirectory(prefix="soap_mi355_") as folder:
         (Path(folder) / "library.so").symlink_to(Path(library).resolve())

@@ -198,6 +198,15 @@ def test_the_build_sees_a_load_that_does_not_wait(written, wait, jump, found):
     assert len(build.unsettled_loads(LISTING.format(written=written, wait=wait, jump=jump))) == found
 
 
+@pytest.mark.parametrize("writer,found", [
+    ("v_readlane_b32 s3, v1, 0", 1), ("v_cmp_gt_i32_e64 s[2:3], v1, s8", 1), ("v_cmp_gt_i32_e32 vcc, s2, v1", 0),
+    ("v_mad_u64_u32 v[4:5], s[2:3], s0, v1, v[6:7]", 1), ("v_add_co_u32 v1, s[8:9], v2, v3", 1), ("v_add_u32_e32 v1, s8, v2", 0),
+    ("s_add_i32 s8, s9, 4", 0)])
+def test_the_build_sees_every_kind_of_writer(writer, found):
+    line = LISTING.format(written=2, wait="s_nop 0", jump=4).replace("v_readfirstlane_b32 s2, v1", writer)
+    assert len(build.unsettled_loads(line)) == found
+
+
 def test_no_load_of_the_library_reads_a_register_too_soon():
     assert build.check_loads(_native.LIBRARY_PATH) > 100
 
