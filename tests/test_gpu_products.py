@@ -1002,3 +1002,124 @@ def test_the_norms_would_show_sums_in_16_bits(device):
             for first in range(0, tokens, 64):
                 total = (total + torch.mm(dy[first:first + 64].t(), x[first:first + 64])).to(kept).float()
             assert (total.double() - expected).norm() > 8 * 2.0 ** -23 * (tokens / 2) ** 0.5 * expected.norm()
+
+
+# ---- further from the ordinary -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("stride_bytes", [(2 << 20) - 4096, 2 << 20, (8 << 20) - 4096, 8 << 20])
+def test_rows_megabytes_apart(device, dtype, stride_bytes):
+    """Around the distances beyond which rows are no longer fetched straight to LDS (2 MiB; for sums 8 MiB)."""
+    stride = stride_bytes // torch.finfo(dtype).bits * 8
+    tokens, outputs, inputs = 290, 130, 72
+
+    def far(seed, rows, columns):
+        view = torch.empty(rows * stride, dtype=dtype, device=device).as_strided((rows, columns), (stride, 1))
+        return view.copy_(values(device, seed, rows, columns, dtype=dtype))
+
+    x, dy = far(1, tokens, inputs), far(2, tokens, outputs)
+    w = far(3, outputs, inputs)
+    check_layer(device, dtype, tokens, 1, outputs, inputs, seed=4, x=x, dy=dy, weights=w[None])
+    out = torch.empty(tokens * stride, dtype=dtype, device=device).as_strided((tokens, outputs), (stride, 1))
+    assert torch.equal(products.expert_product(x, w, None, out=out), products.expert_product(x, w, None))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("tokens,experts", [(3000, 5000), (40, 1000), (20000, 200)])
+def test_many_experts(device, dtype, tokens, experts):
+    check_layer(device, dtype, tokens, experts, 24, 40, seed=7, spare=3)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("tokens,experts,outputs,inputs", [(0, 2, 8, 16), (5, 0, 8, 16), (5, 2, 0, 16), (5, 2, 8, 0)])
+def test_expert_linear_of_empty_extents(device, checkpoint, tokens, experts, outputs, inputs):
+    x = torch.ones(tokens, inputs, device=device, requires_grad=True)
+    weights = torch.ones(experts, outputs, inputs, device=device, requires_grad=True)
+    ends = torch.full((experts,), tokens, dtype=torch.int64, device=device)
+    y = products.expert_linear(x, weights, ends, checkpoint=checkpoint)
+    assert y.shape == (tokens, outputs) and not y.any()
+    y.backward(torch.ones_like(y))
+    assert x.grad.shape == x.shape and not x.grad.any()
+    assert weights.grad.shape == weights.shape and not weights.grad.any()
+
+
+def test_calls_from_two_threads(device):
+    """Each thread on a stream of its own, with other sizes, among them refused calls."""
+    import threading
+
+    def inputs(seed, tokens):
+        return (values(device, seed, tokens, 256, dtype=torch.bfloat16), values(device, seed + 1, 4, 192, 256, dtype=torch.bfloat16),
+                values(device, seed + 2, tokens, 192, dtype=torch.bfloat16), split(tokens, 4, device, seed)[1])
+
+    def work(x, weights, dy, ends, plan, stream, into):
+        with torch.cuda.device(device), torch.cuda.stream(stream):
+            for _ in range(20):
+                into.append(_pass(x, weights, dy, ends, plan))
+                try:
+                    products.expert_product(x, weights[:, :, :x.shape[0] % 200], ends)
+                except ValueError as error:
+                    into.append(str(error))
+
+    cases, expected, found, threads = [], [], [], []
+    for seed, tokens in ((1, 300), (20, 411)):
+        case = inputs(seed, tokens)
+        plan = products.quantize_tokens(case[1][0])
+        cases.append((*case, plan))
+        expected.append(_pass(*case, plan))
+    torch.cuda.synchronize(device)
+    for case in cases:
+        found.append([])
+        threads.append(threading.Thread(target=work, args=(*case, torch.cuda.Stream(device=device), found[-1])))
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize(device)
+    for case, results, wanted in zip(cases, found, expected):
+        assert len(results) == 40
+        message = f"x has 256 columns, expected {case[0].shape[0] % 200}."
+        for result in results:
+            if isinstance(result, str):
+                assert result == message
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(result, wanted))
+
+
+def test_mixed_training_pass_captured_and_replayed(device):
+    """Forward and backward pass under autocast in one graph: float32 weights, changed between the replays."""
+    tokens, experts, outputs, inputs = 150, 4, 40, 136
+    x, dy = torch.zeros(tokens, inputs, device=device), torch.zeros(tokens, outputs, dtype=torch.bfloat16, device=device)
+    weights = torch.zeros(experts, outputs, inputs, device=device)
+    ends = torch.zeros(experts, dtype=torch.int64, device=device)
+    leaves = x.requires_grad_(), weights.requires_grad_()
+
+    def fill(seed):
+        with torch.no_grad():
+            x.copy_(values(device, seed, tokens, inputs, dtype=torch.float32))
+            dy.copy_(values(device, seed + 1, tokens, outputs, dtype=torch.bfloat16))
+            weights.copy_(values(device, seed + 2, experts, outputs, inputs, dtype=torch.float32))
+            ends.copy_(split(tokens, experts, device, seed, spare=seed)[1])
+
+    def eager():
+        with torch.no_grad():
+            rows, matrices = x.bfloat16(), weights.bfloat16()
+            saved = products.checkpoint_activations(rows)
+            return (products.expert_product(rows, matrices, ends), products.expert_input_gradient(dy, matrices, ends).float(),
+                    products.expert_weight_gradient(dy, saved, ends))
+
+    fill(0)
+    eager()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with torch.autocast("cuda", dtype=torch.bfloat16, cache_enabled=False):
+            y = products.expert_linear(x, weights, ends, checkpoint=True)
+        captured = torch.autograd.grad(y, leaves, dy)
+        y = y.detach()
+    for seed in (3, 11, 20):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        for actual, expected in zip((y, *captured), eager()):
+            assert torch.equal(actual, expected)
